@@ -418,6 +418,66 @@ int tbcompat_upSample(tb_ctx* ctx, int64_t aBatch, int64_t aChannels, int64_t ou
 int tb_bn_fwd(tb_ctx* ctx, int64_t batch, int64_t channels, int64_t spatial, const float* x, const float* mean,
               const float* variance, const float* scales, const float* biases, float* y);
 
+/* ---- int8 connected layer and token log probabilities ---------------------------------------
+ * The head of a network that answers with one of many tokens: TConnectedLayer with int8 operands
+ * (a scale for each token, i.e. row of x, and for each output channel) and what a program reads
+ * off its logits. The reference has neither; these entry points are new. Matrices are row-major
+ * with a row stride in elements, at least the row's length unless there is one row; x, y and logits
+ * are of a TB_* element type and need no alignment beyond their element's. Nothing outside the
+ * rows is read or written. Zero rows are a valid call that does nothing. */
+#define TB_F32  0
+#define TB_BF16 1
+#define TB_F16  2
+
+/* codes[i][j] = rint(x[i][j] * (127 / amax_i)), scales[i] = amax_i / 127, with
+ * amax_i = max(max_j |x[i][j]|, 2^-100), every operation rounded to single once (ties of rint to
+ * even). A row that holds a NaN or an infinity gets codes 0 and a NaN scale, so every product
+ * with it is NaN. x_stride may be 0 (one row for all). Quantizes activations by token, and
+ * [outputs][inputs] weights by output channel. */
+int tb_quantize_rows(tb_ctx* ctx, int64_t rows, int64_t cols, const void* x, int64_t x_type, int64_t x_stride,
+                     int8_t* codes, int64_t code_stride, float* scales);
+
+/* y[i][j] = act((sum_l a[i][l] * w[j][l]) * (a_scales[i] * w_scales[j]) + bias[j]) for i < m, j < n:
+ * the sum exact in int32 (k <= 131071), each later operation rounded to single, y rounded once to
+ * its type. bias may be NULL. a and w start on 16 bytes and their strides are multiples of 16
+ * (codes may hold -128; what stands between k and the stride is not used). */
+int tb_int8_gemm(tb_ctx* ctx, int64_t m, int64_t n, int64_t k, const int8_t* a, int64_t a_stride,
+                 const float* a_scales, const int8_t* w, int64_t w_stride, const float* w_scales,
+                 const float* bias, int64_t activation, void* y, int64_t y_type, int64_t y_stride);
+
+/* tb_quantize_rows of x, then tb_int8_gemm, without the caller's buffers for the codes (they are
+ * in the context's workspace, or in shared memory for a few tokens). Same results. */
+int tb_int8_connected_fwd(tb_ctx* ctx, int64_t m, int64_t n, int64_t k, const void* x, int64_t x_type,
+                          int64_t x_stride, const int8_t* w, int64_t w_stride, const float* w_scales,
+                          const float* bias, int64_t activation, void* y, int64_t y_type, int64_t y_stride);
+
+/* For each row of logits, with z = logits / temperature and the row's softmax p:
+ *   row_max[i] = max_j logits_j, log_sum[i] = log sum_j exp(z_j - row_max / temperature),
+ *   lse[i] = row_max / temperature + log_sum, logprob[i] = log p[tokens[i]], entropy[i] = -sum_j p_j log p_j,
+ *   top_token[i][0..top) the columns of the largest logits in descending order (equal logits: the
+ *   lowest column first), top_logprob[i][..] their log probabilities.
+ * top <= min(32, vocab); 0 leaves the last two out. tokens may be NULL (logprob is then left out); a
+ * row whose token is negative has logprob 0, one whose token is >= vocab NaN. A logit of -infinity is
+ * masked: probability 0. A row with nothing left has row_max, lse and log probabilities -infinity,
+ * log_sum and entropy 0; one that holds a NaN or +infinity has NaN everywhere and top tokens -1.
+ * entropy, lse, row_max and log_sum may be NULL. */
+int tb_token_logprobs_fwd(tb_ctx* ctx, int64_t rows, int64_t vocab, const void* logits, int64_t type,
+                          int64_t stride, const int64_t* tokens, float temperature, int64_t top,
+                          float* logprob, float* entropy, float* lse, float* row_max, float* log_sum,
+                          float* top_logprob, int64_t* top_token);
+
+/* Gradient of sum_i g_logprob[i] * logprob[i] + g_entropy[i] * entropy[i] with respect to the
+ * logits, from the row_max, log_sum and (with g_entropy) entropy that tb_token_logprobs_fwd gave (not
+ * from lse, which has no room for log_sum beside large logits):
+ *   d[i][j] = (g_logprob * ((j == token) - p_j) - g_entropy * p_j * (log p_j + entropy)) / temperature
+ * rounded once to the logits' type. Either g may be NULL (0). A negative token leaves g_logprob out;
+ * masked columns other than the token and rows with nothing left get 0; rows with NaN, and with a
+ * token >= vocab unless g_logprob is NULL, get NaN. dlogits may be logits itself (same stride). */
+int tb_token_logprobs_bwd(tb_ctx* ctx, int64_t rows, int64_t vocab, const void* logits, int64_t type,
+                          int64_t stride, const int64_t* tokens, float temperature, const float* row_max,
+                          const float* log_sum, const float* entropy, const float* g_logprob, const float* g_entropy,
+                          void* dlogits, int64_t d_stride);
+
 /* ---- multi-GPU group (NCCL) ------------------------------------------------------------
  * Inference shards by image: each GPU runs the whole network on its slice of the batch, and the
  * only exchange is the final gather of per-GPU results (detection records, counts, logits) to

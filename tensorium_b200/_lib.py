@@ -32,6 +32,8 @@ MATH_TF32 = 1
 MATH_FP32_TILED = 2  # FP32 with the summation reordered (tiles, split-K): not bit-exact
 MATH_BF16_SPLIT = 3  # tensor cores on bf16 (hi, lo) operand pairs, networks only
 
+F32_ELEM, BF16_ELEM, F16_ELEM = 0, 1, 2  # TB_F32, TB_BF16, TB_F16
+
 XNOR_PAD_BIT0 = 0
 XNOR_PAD_ZERO = 1
 
@@ -174,6 +176,11 @@ SIGNATURES = {
     "tb_fc_fwd": [P, I64, I64, I64, P, P, P, I64, P],
     "tb_softmax_fwd": [P, I64, I64, I64, F32, P, P],
     "tb_avgpool_fwd": [P, I64, I64, I64, I64, P, P],
+    "tb_quantize_rows": [P, I64, I64, P, I64, I64, P, I64, P],
+    "tb_int8_gemm": [P, I64, I64, I64, P, I64, P, P, I64, P, P, I64, P, I64, I64],
+    "tb_int8_connected_fwd": [P, I64, I64, I64, P, I64, I64, P, I64, P, P, I64, P, I64, I64],
+    "tb_token_logprobs_fwd": [P, I64, I64, P, I64, I64, P, F32, I64, P, P, P, P, P, P, P],
+    "tb_token_logprobs_bwd": [P, I64, I64, P, I64, I64, P, F32, P, P, P, P, P, P, I64],
     "tb_net_create": [P, I64, I64, I64, I64, C.POINTER(P)],
     "tb_net_destroy": [P],
     "tb_net_add_conv": [P, I64, I64, I64, I64, I64, I64, P, P, P, P, P],

@@ -35,6 +35,11 @@ class Context:
         check(lib.tb_set_stream(self.handle, C.c_void_p(raw)))
         self.stream = stream
 
+    @property
+    def raw_stream(self) -> int:
+        """cudaStream_t that the context launches on (0: the legacy default stream)."""
+        return lib.tb_get_stream(self.handle) or 0
+
     def sync(self) -> None:
         check(lib.tb_sync(self.handle))
 

@@ -15,6 +15,9 @@ fp32 torch tensors on the context's GPU (TSingleTensor.devData).
     TConnectedLayer       source/nconnectedlayer.pas:62-66, 157-184
     TSoftmaxLayer         source/nsoftmaxlayer.pas:49-52, 139-167
     TAvgPoolLayer         source/navgpoollayer.pas:27-30, 60-84
+
+TInt8ConnectedLayer and TTokenLogprobsLayer have no counterpart there: the connected layer on int8
+weights, and the log probabilities read off its outputs where a TSoftmaxLayer would follow.
 """
 from __future__ import annotations
 
@@ -25,7 +28,7 @@ from typing import Optional
 import numpy as np
 import torch
 
-from . import synth
+from . import synth, tokens
 from ._lib import ACT, XNOR_PAD_BIT0, ConvDesc, Detection, YoloHead, check, lib
 from .context import Context, ptr
 
@@ -337,6 +340,52 @@ class TConnectedLayer(TBaseLayer):
                             ptr(self._dev[0]), ptr(self._dev[1]), self.ActivationType, ptr(y)))
         self.output = y
         return y
+
+
+class TInt8ConnectedLayer(TBaseLayer):
+    """TConnectedLayer with int8 weights, a scale for each output, and inputs quantized token by
+    token on the way in (tokens.int8_connected). x: [tokens, AInputs] of any float type; the output
+    has its type."""
+
+    def __init__(self, AInputs, aOutputs, AActivationType="linear", weights=None, biases=None):
+        self.inputs, self.outputs = AInputs, aOutputs
+        self.ActivationType = _act(AActivationType)
+        self.weights = weights if weights is not None else np.zeros((aOutputs, AInputs), np.float32)
+        self.biases = biases  # float32 [aOutputs] or None
+        self._dev = None
+
+    def upload(self, ctx: Context = None):
+        """Quantize the weights on the GPU, once, by output channel."""
+        if ctx is not None:
+            self.bind(ctx)
+        w = self.weights
+        w = w.to(self.ctx.torch_device) if isinstance(w, torch.Tensor) else _dev(self.ctx, w)
+        codes, scales = tokens.quantize_rows(self.ctx, w)
+        self._dev = (codes, scales, None if self.biases is None else _dev(self.ctx, self.biases))
+
+    def forward(self, state: TNNetState):
+        if self._dev is None:
+            self.upload()
+        codes, scales, biases = self._dev
+        self.output = tokens.int8_connected(self.ctx, state.input, codes, scales, biases, self.ActivationType)
+        return self.output
+
+
+class TTokenLogprobsLayer(TBaseLayer):
+    """Log probabilities of given tokens, entropies and the `top` most probable tokens of logits
+    [rows, vocab] (tokens.token_logprobs), and their gradient."""
+
+    def __init__(self, top=0, temperature=1.0):
+        self.top, self.temperature = top, temperature
+
+    def forward(self, state: TNNetState, given: Optional[torch.Tensor] = None):
+        self.output = tokens.token_logprobs(self.ctx, state.input, given, self.top, self.temperature)
+        return self.output
+
+    def backward(self, state: TNNetState, given, grad_logprobs=None, grad_entropy=None, out=None):
+        """Gradient with respect to state.input, after forward on the same state and tokens."""
+        return tokens.token_logprobs_backward(self.ctx, state.input, given, self.output, grad_logprobs, grad_entropy,
+                                              self.temperature, out)
 
 
 class TSoftmaxLayer(TBaseLayer):
