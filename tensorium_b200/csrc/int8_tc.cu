@@ -84,8 +84,30 @@ template <typename T> struct Channel {
         bias = in && p.bias ? __ldg(p.bias + ch) : 0.f;
         y = static_cast<T*>(p.y) + ch;
     }
-    __device__ __forceinline__ void store(const Int8Args& p, int64_t token, float a_scale, int acc) const {
-        y[token * p.y_stride] = Elem<T>::put(int8_epilogue(acc, __fmul_rn(a_scale, scale), bias, p.bias != nullptr, p.act));
+    // N consecutive tokens from `token`: every value first, then every store, so that the chains of
+    // one thread overlap (an epilogue warp has a scheduler almost to itself)
+    template <int N> __device__ __forceinline__ void store(const Int8Args& p, int64_t token, const float* a_scales, const int* acc) const {
+        float v[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = __fmul_rn(__int2float_rn(acc[i]), __fmul_rn(a_scales[i], scale));
+        if (p.bias) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = __fadd_rn(v[i], bias);
+        }
+        if (p.act != TB_ACT_LINEAR) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = tb_activate_dev(v[i], p.act);
+        }
+        T* to = y + token * p.y_stride;
+        const int64_t left = in ? p.m - token : 0;
+        if (left >= N) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) to[i * p.y_stride] = Elem<T>::put(v[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (i < left) to[i * p.y_stride] = Elem<T>::put(v[i]);
+        }
     }
 };
 
@@ -102,6 +124,7 @@ __global__ void __launch_bounds__(192) k_int8_stream(const __grid_constant__ I8M
     __shared__ __align__(8) uint64_t full_bar[I8_MAX_STAGES], empty_bar[I8_MAX_STAGES], done_bar;
     __shared__ uint32_t tmem_base;
     __shared__ volatile int abort_flag;
+    __shared__ __align__(16) float a_scales[BT];
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int splits = gridDim.z, z = blockIdx.z;
@@ -175,10 +198,12 @@ __global__ void __launch_bounds__(192) k_int8_stream(const __grid_constant__ I8M
     const uint32_t taddr = tmem0 + ((uint32_t)(quarter * 32) << 16);
     bool ok = true;
     if (warp >= 2) {
+        grid_dep_wait();
+        for (int i = ch; i < BT; i += 128) a_scales[i] = m0 + i < p.m ? p.a_scales[m0 + i] : 0.f;
+        asm volatile("bar.sync 1, 128;\n" ::: "memory");
         ok = tc::mbar_wait_bounded(&done_bar, 0, &abort_flag, status, 933);
         ok = __all_sync(0xffffffffu, ok && !abort_flag);
         tc::tc_fence_after();
-        grid_dep_wait();  // a_scales
     }
     if (splits == 1) {
         if (warp >= 2 && ok) {
@@ -188,12 +213,7 @@ __global__ void __launch_bounds__(192) k_int8_stream(const __grid_constant__ I8M
                 uint32_t r[16];
                 tc::tmem_ld16_issue(taddr + c0, r);
                 tc::tmem_wait16(r);
-                const float sa = m0 + c0 + (lane & 15) < p.m ? p.a_scales[m0 + c0 + (lane & 15)] : 0.f;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float s = __shfl_sync(0xffffffffu, sa, i);
-                    if (c.in && m0 + c0 + i < p.m) c.store(p, m0 + c0 + i, s, (int)r[i]);
-                }
+                c.template store<16>(p, m0 + c0, a_scales + c0, reinterpret_cast<int*>(r));
             }
         }
     } else {
@@ -221,12 +241,12 @@ __global__ void __launch_bounds__(192) k_int8_stream(const __grid_constant__ I8M
         if (warp >= 2 && ok) {
             const Channel<T> c(p, n0 + ch);
             const int* buf = reinterpret_cast<const int*>(smem_raw + (red - (unsigned)__cvta_generic_to_shared(smem_raw))) + ch;
-            for (int i = 0; i < share; ++i) {
-                const int64_t token = m0 + z * share + i;
-                if (token >= p.m) break;
-                int acc = 0;
-                for (int s = 0; s < splits; ++s) acc += buf[(s * share + i) * 128];
-                if (c.in) c.store(p, token, p.a_scales[token], acc);
+            for (int i = 0; i < share; i += 2) {  // shares are powers of two from 2 on
+                int acc[2] = {0, 0};
+#pragma unroll 4
+                for (int s = 0; s < splits; ++s)
+                    for (int u = 0; u < 2; ++u) acc[u] += buf[(s * share + i + u) * 128];
+                c.template store<2>(p, m0 + z * share + i, a_scales + z * share + i, acc);
             }
         }
     }
@@ -254,6 +274,7 @@ __global__ void __launch_bounds__(I8P_THREADS, 1) k_int8_pair(const __grid_const
     __shared__ __align__(8) uint64_t full_bar[I8P_STAGES], empty_bar[I8P_STAGES], tfull_bar[2], tempty_bar[2], drain_bar;
     __shared__ uint32_t tmem_base;
     __shared__ volatile int abort_flag;
+    __shared__ __align__(16) float a_scales[8][128];  // each epilogue warp's tokens
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = (int)tc::cluster_rank();
@@ -348,23 +369,22 @@ __global__ void __launch_bounds__(I8P_THREADS, 1) k_int8_pair(const __grid_const
             int64_t mt, nt;
             i8p_tile(t, tiles_m, tiles_n, &mt, &nt);
             const int buf = tl & 1, u = tl >> 1;
+            const int64_t m0 = mt * 256 + half * 128;
+            float* sa = a_scales[warp - 2];
+            __syncwarp();
+            for (int i = lane; i < 128; i += 32) sa[i] = m0 + i < p.m ? p.a_scales[m0 + i] : 0.f;
+            __syncwarp();
             const bool ok = !abort_flag && tc::mbar_wait_bounded(&tfull_bar[buf], u & 1, &abort_flag, status, 944);
             if (tc::epi_any(!ok)) break;  // tcgen05.ld is warp-collective: the epilogue warps leave together
             tc::tc_fence_after();
             const Channel<T> c(p, nt * 256 + rank * 128 + quarter * 32 + lane);
-            const int64_t m0 = mt * 256 + half * 128;
             const uint32_t taddr = tmem0 + buf * 256 + half * 128 + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll 1
             for (int c0 = 0; c0 < 128; c0 += 16) {
                 uint32_t r[16];
                 tc::tmem_ld16_issue(taddr + c0, r);
                 tc::tmem_wait16(r);
-                const float sa = m0 + c0 + (lane & 15) < p.m ? p.a_scales[m0 + c0 + (lane & 15)] : 0.f;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float s = __shfl_sync(0xffffffffu, sa, i);
-                    if (c.in && m0 + c0 + i < p.m) c.store(p, m0 + c0 + i, s, (int)r[i]);
-                }
+                c.template store<16>(p, m0 + c0, sa + c0, reinterpret_cast<int*>(r));
             }
             tc::tc_fence_before();
             __syncwarp();
