@@ -3,10 +3,15 @@
 // first two (tb_token_logprobs_bwd).
 #include "elem.cuh"
 
+#include <algorithm>
+#include <cstring>
+
 namespace tbi {
 namespace {
 
 constexpr int TOP_MAX = 32;
+
+struct Part;
 
 struct LogprobArgs {
     int64_t rows, vocab;
@@ -22,90 +27,463 @@ struct LogprobArgs {
     float* log_sum;
     float* top_logprob;
     int64_t* top_token;
+    int splits;            // parts of a row, joined by the last of their CTAs to finish
+    Part* parts;
+    int* counters;         // finished parts of each row, left at 0
 };
 
 __device__ __forceinline__ float nan_f() { return __uint_as_float(0x7fffffffu); }
 
+__device__ __forceinline__ uint32_t ordered(float v) {
+    const uint32_t u = __float_as_uint(v + 0.f);
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float unordered(uint32_t u) { return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u); }
+
 // Order of alternatives as one unsigned key: the value's order in the high half (-0 counts as 0), then
 // the lower column first. 0 is below every key.
 __device__ __forceinline__ unsigned long long top_key(float v, uint32_t col) {
-    uint32_t u = __float_as_uint(v + 0.f);
-    u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-    return ((unsigned long long)u << 32) | (uint32_t)~col;
+    return ((unsigned long long)ordered(v) << 32) | (uint32_t)~col;
 }
 __device__ __forceinline__ uint32_t key_col(unsigned long long k) { return ~(uint32_t)k; }
-__device__ __forceinline__ float key_val(unsigned long long k) {
-    const uint32_t u = (uint32_t)(k >> 32);
-    return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
+__device__ __forceinline__ float key_val(unsigned long long k) { return unordered((uint32_t)(k >> 32)); }
+
+// ---- arithmetic on two floats at a time ---------------------------------------------------------
+struct F2 {
+    float x, y;
+};
+__device__ __forceinline__ unsigned long long f2_bits(F2 a) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.x), "f"(a.y));
+    return r;
+}
+__device__ __forceinline__ F2 f2_of(unsigned long long b) {
+    F2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(b));
+    return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
+    return f2_of(r);
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
+    return f2_of(r);
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)), "l"(f2_bits(c)));
+    return f2_of(r);
+}
+// 2^x to about 2^-22; 0 below 2^-126
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
 
-template <typename V, typename F> __device__ V block_reduce(V v, V* part, F f) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = part[0];
-    for (int i = 1; i < (int)blockDim.x / 32; ++i) v = f(v, part[i]);
-    return v;
-}
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+// Exponents are clamped here: 2^-200 is 0 in single precision, and -infinity (a mask) and the NaN of
+// (-infinity) - (-infinity) become a finite number whose product with 0 is 0.
+constexpr float EXP_FLOOR = -200.f;
 
-// One CTA per row, a pass for the maximum, one for the sums and one for each alternative.
-template <typename T> __global__ void __launch_bounds__(256) k_token_logprobs(const LogprobArgs p) {
-    TB_GRID_DEP_ENTRY();
-    __shared__ float part[8];
-    __shared__ unsigned long long kpart[8];
-    const int64_t row = blockIdx.x;
-    const T* x = static_cast<const T*>(p.logits) + row * p.stride;
-    float m = -INFINITY;
-    bool bad = false;
-    for (int64_t i = threadIdx.x; i < p.vocab; i += blockDim.x) {
-        const float v = Elem<T>::get(x[i]);
-        bad |= !(v < INFINITY);
-        m = fmaxf(m, v);
+// ---- 16 bytes of logits -----------------------------------------------------------------------
+template <typename T> struct Chunk;
+template <> struct Chunk<float> {
+    static constexpr uint32_t MASKED = 0xff800000u;  // -infinity
+    static __device__ __forceinline__ float vmax(const uint4& r) {
+        return max_nan(max_nan(__uint_as_float(r.x), __uint_as_float(r.y)), max_nan(__uint_as_float(r.z), __uint_as_float(r.w)));
     }
-    m = block_reduce(m, part, [](float a, float b) { return fmaxf(a, b); });
-    bad = __syncthreads_or(bad);
-    const bool empty = m == -INFINITY;
-    float z = 0.f, s = 0.f;
-    if (!bad && !empty)
-        for (int64_t i = threadIdx.x; i < p.vocab; i += blockDim.x) {
-            const float t = fmaxf(__fmul_rn(__fsub_rn(Elem<T>::get(x[i]), m), p.inv_t), -200.f);
-            const float e = expf(t);
-            z += e;
-            s = fmaf(e, t, s);
+    static __device__ __forceinline__ void get(const uint4& r, F2* f) {
+        f[0] = {__uint_as_float(r.x), __uint_as_float(r.y)};
+        f[1] = {__uint_as_float(r.z), __uint_as_float(r.w)};
+    }
+    static __device__ __forceinline__ uint4 put(const F2* f) {
+        return make_uint4(__float_as_uint(f[0].x), __float_as_uint(f[0].y), __float_as_uint(f[1].x), __float_as_uint(f[1].y));
+    }
+};
+template <> struct Chunk<__nv_bfloat16> {
+    static constexpr uint32_t MASKED = 0xff80ff80u;
+    static __device__ __forceinline__ float vmax(const uint4& r) {
+        auto h = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
+        const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h(r.x), h(r.y)), __hmax2_nan(h(r.z), h(r.w)));
+        return max_nan(__low2float(m), __high2float(m));
+    }
+    static __device__ __forceinline__ F2 two(uint32_t w) { return {__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)}; }
+    static __device__ __forceinline__ void get(const uint4& r, F2* f) { f[0] = two(r.x), f[1] = two(r.y), f[2] = two(r.z), f[3] = two(r.w); }
+    static __device__ __forceinline__ uint32_t one(F2 a) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a.x, a.y);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ uint4 put(const F2* f) { return make_uint4(one(f[0]), one(f[1]), one(f[2]), one(f[3])); }
+};
+template <> struct Chunk<__half> {
+    static constexpr uint32_t MASKED = 0xfc00fc00u;
+    static __device__ __forceinline__ float vmax(const uint4& r) {
+        auto h = [](uint32_t w) { return *reinterpret_cast<const __half2*>(&w); };
+        const __half2 m = __hmax2_nan(__hmax2_nan(h(r.x), h(r.y)), __hmax2_nan(h(r.z), h(r.w)));
+        return max_nan(__low2float(m), __high2float(m));
+    }
+    static __device__ __forceinline__ F2 two(uint32_t w) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+        return {f.x, f.y};
+    }
+    static __device__ __forceinline__ void get(const uint4& r, F2* f) { f[0] = two(r.x), f[1] = two(r.y), f[2] = two(r.z), f[3] = two(r.w); }
+    static __device__ __forceinline__ uint32_t one(F2 a) {
+        const __half2 h = __floats2half2_rn(a.x, a.y);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ uint4 put(const F2* f) { return make_uint4(one(f[0]), one(f[1]), one(f[2]), one(f[3])); }
+};
+
+// A row as 16-byte chunks from the 16-byte boundary at or before its start: chunk v holds columns
+// v * E - head .. Whole chunks are one access; the first and last, where the row covers them in part, go element
+// by element, with -infinity in the other places. Nothing outside the row is touched.
+template <typename T> struct Row {
+    static constexpr int E = 16 / sizeof(T);
+    const T* base;  // of chunk 0, before the row's start by `head` elements
+    int head, end;  // the row's columns are elements head .. end - 1 of the chunks
+    __device__ __forceinline__ Row(const T* x, int64_t vocab) {
+        head = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+        base = reinterpret_cast<const T*>(reinterpret_cast<uintptr_t>(x) & ~(uintptr_t)15);
+        end = head + (int)vocab;
+    }
+    __device__ __forceinline__ int chunks() const { return (int)(((int64_t)end + E - 1) / E); }
+    __device__ __forceinline__ bool whole(int v) const { return v * (int64_t)E >= head && (v + 1) * (int64_t)E <= end; }
+    __device__ __forceinline__ uint4 load(int v, int stop) const {
+        if (v < stop && whole(v)) return *reinterpret_cast<const uint4*>(base + (int64_t)v * E);
+        uint4 r = make_uint4(Chunk<T>::MASKED, Chunk<T>::MASKED, Chunk<T>::MASKED, Chunk<T>::MASKED);
+        if (v < stop) {
+            T t[E];
+            memcpy(t, &r, 16);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int64_t i = (int64_t)v * E + e;
+                if (i >= head && i < end) t[e] = base[i];
+            }
+            memcpy(&r, t, 16);
         }
-    z = block_reduce(z, part, [](float a, float b) { return a + b; });
-    s = block_reduce(s, part, [](float a, float b) { return a + b; });
-    const float logz = logf(z);
+        return r;
+    }
+};
+
+// ---- the most probable tokens -------------------------------------------------------------------
+// A warp keeps its best keys sorted, the i-th best in lane i (0: none yet).
+// 32 values, one a lane, into descending order
+template <typename K> __device__ __forceinline__ K sort32(K a, int lane) {
+#pragma unroll
+    for (int n = 2; n <= 32; n *= 2)
+#pragma unroll
+        for (int o = n / 2; o; o /= 2) {
+            const K b = __shfl_xor_sync(0xffffffffu, a, o);
+            const bool up = ((lane & n) == 0) == ((lane & o) == 0);  // this lane keeps the larger one
+            a = up == (a > b) ? a : b;
+        }
+    return a;
+}
+// the 32 largest of two descending lists, descending
+template <typename K> __device__ __forceinline__ K merge32(K a, K b, int lane) {
+    b = __shfl_xor_sync(0xffffffffu, b, 31);
+    a = a > b ? a : b;
+#pragma unroll
+    for (int o = 16; o; o /= 2) {
+        b = __shfl_xor_sync(0xffffffffu, a, o);
+        a = ((lane & o) == 0) == (a > b) ? a : b;
+    }
+    return a;
+}
+// the lists of all warps of the CTA into warp 0's (every thread calls it)
+template <int NW, typename K> __device__ __forceinline__ K merge_warps(K a, K (*buf)[32], int warp, int lane) {
+#pragma unroll
+    for (int n = NW / 2; n; n /= 2) {
+        if (warp >= n && warp < 2 * n) buf[warp][lane] = a;
+        __syncthreads();
+        if (warp < n) a = merge32(a, buf[warp + n][lane], lane);
+    }
+    return a;
+}
+// one key for the whole warp into a list of `top`
+__device__ __forceinline__ unsigned long long insert(unsigned long long list, unsigned long long key, int lane) {
+    const int at = __popc(__ballot_sync(0xffffffffu, list > key));
+    const unsigned long long up = __shfl_up_sync(0xffffffffu, list, 1);
+    return lane < at ? list : lane == at ? key : up;
+}
+
+// ---- forward --------------------------------------------------------------------------------------
+// Sums of a part of a row: sum 2^t and sum t 2^t over t = (logit - max) * c, c = log2(e) / temperature.
+struct Sums {
+    float max, z, s;
+    int bad;  // a NaN or +infinity is among the logits
+};
+__device__ __forceinline__ Sums join(const Sums& a, const Sums& b, float c) {
+    Sums r;
+    r.max = fmaxf(a.max, b.max);
+    const float da = fmaxf(__fmul_rn(__fsub_rn(a.max, r.max), c), EXP_FLOOR), db = fmaxf(__fmul_rn(__fsub_rn(b.max, r.max), c), EXP_FLOOR);
+    const float fa = exp2_fast(da), fb = exp2_fast(db);
+    r.z = fmaf(a.z, fa, __fmul_rn(b.z, fb));
+    r.s = fmaf(fmaf(a.z, da, a.s), fa, __fmul_rn(fmaf(b.z, db, b.s), fb));
+    r.bad = a.bad | b.bad;
+    return r;
+}
+__device__ __forceinline__ Sums join_warp(Sums a, float c) {
+#pragma unroll
+    for (int o = 16; o; o /= 2) {
+        Sums b;
+        b.max = __shfl_xor_sync(0xffffffffu, a.max, o);
+        b.z = __shfl_xor_sync(0xffffffffu, a.z, o);
+        b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
+        b.bad = __shfl_xor_sync(0xffffffffu, a.bad, o);
+        a = join(a, b, c);
+    }
+    return a;
+}
+
+// What a split of a row leaves in the workspace for the one that joins them.
+struct Part {
+    Sums sums;
+    unsigned long long keys[TOP_MAX];
+};
+
+// Results of one row, by one warp that holds its sums and its best keys.
+template <typename T>
+__device__ __forceinline__ void write_row(const LogprobArgs& p, int64_t row, const Sums& a, unsigned long long list, float given, int lane) {
+    const bool empty = a.max == -INFINITY;
+    const float logz = logf(a.z);
     auto logprob = [&](float v) {
-        return bad ? nan_f() : empty ? -INFINITY : __fsub_rn(__fmul_rn(__fsub_rn(v, m), p.inv_t), logz);
+        return a.bad ? nan_f() : empty ? -INFINITY : __fsub_rn(__fmul_rn(__fsub_rn(v, a.max), p.inv_t), logz);
     };
-    if (threadIdx.x == 0) {
+    if (lane == 0) {
         if (p.logprob) {
             const int64_t t = p.tokens[row];
-            p.logprob[row] = t < 0 ? (bad ? nan_f() : 0.f) : t >= p.vocab ? nan_f() : logprob(Elem<T>::get(x[t]));
+            p.logprob[row] = t >= p.vocab ? nan_f() : t < 0 ? (a.bad ? nan_f() : 0.f) : logprob(given);
         }
-        if (p.entropy) p.entropy[row] = bad ? nan_f() : empty ? 0.f : fmaxf(__fsub_rn(logz, __fdiv_rn(s, z)), 0.f);
-        if (p.row_max) p.row_max[row] = bad ? nan_f() : m;
-        if (p.log_sum) p.log_sum[row] = bad ? nan_f() : empty ? 0.f : logz;
-        if (p.lse) p.lse[row] = bad ? nan_f() : empty ? -INFINITY : __fadd_rn(__fmul_rn(m, p.inv_t), logz);
+        if (p.entropy)
+            p.entropy[row] = a.bad ? nan_f() : empty ? 0.f : fmaxf(__fsub_rn(logz, __fmul_rn(__fdiv_rn(a.s, a.z), LN2)), 0.f);
+        if (p.lse) p.lse[row] = a.bad ? nan_f() : empty ? -INFINITY : __fadd_rn(__fmul_rn(a.max, p.inv_t), logz);
+        if (p.row_max) p.row_max[row] = a.bad ? nan_f() : a.max;
+        if (p.log_sum) p.log_sum[row] = a.bad ? nan_f() : empty ? 0.f : logz;
     }
-    unsigned long long last = ~0ull;
-    for (int r = 0; r < p.top; ++r) {
-        unsigned long long best = 0;
-        for (int64_t i = threadIdx.x; i < p.vocab; i += blockDim.x) {
-            const unsigned long long k = top_key(Elem<T>::get(x[i]), (uint32_t)i);
-            if (k < last && k > best) best = k;
+    if (p.top == 0) return;
+    const int have = min(__popc(__ballot_sync(0xffffffffu, list != 0)), p.top);
+    if (have < p.top) {
+        // Fewer columns than alternatives are not masked, and all of those are in the list: the lowest
+        // masked columns follow. They are among the first 64, of which the list holds at most 31.
+        bool in0 = lane >= p.vocab, in1 = lane + 32 >= p.vocab;
+        for (int i = 0; i < have; ++i) {
+            const uint32_t col = key_col(__shfl_sync(0xffffffffu, list, i));
+            in0 |= col == (uint32_t)lane;
+            in1 |= col == (uint32_t)lane + 32;
         }
-        last = block_reduce(best, kpart, [](unsigned long long a, unsigned long long b) { return a > b ? a : b; });
-        if (threadIdx.x == 0) {
-            p.top_token[row * p.top + r] = bad ? -1 : (int64_t)key_col(last);
-            p.top_logprob[row * p.top + r] = logprob(key_val(last));
-        }
+        unsigned long long left = __ballot_sync(0xffffffffu, !in0) | (unsigned long long)__ballot_sync(0xffffffffu, !in1) << 32;
+        for (int i = have; i < lane; ++i) left &= left - 1;  // the (lane - have)-th of them
+        if (lane >= have) list = top_key(-INFINITY, (uint32_t)(__ffsll((long long)left) - 1));
+    }
+    if (lane < p.top) {
+        p.top_token[row * p.top + lane] = a.bad ? -1 : (int64_t)key_col(list);
+        p.top_logprob[row * p.top + lane] = logprob(key_val(list));
     }
 }
 
+// One pass over the logits. NW warps work on a row (1: a warp has a row to itself, four in a CTA), or
+// on one of `splits` parts of a row where the rows alone do not fill the GPU.
+//
+// Sums: each thread keeps sum 2^t and sum t 2^t against a reference of its own, an earlier logit,
+// and moves the reference only when a logit is 2^40 above it; the sums are floating point, so nothing is
+// lost below that, and most steps need no new maximum. Alternatives: a step's largest logit per thread
+// is compared with the list's last entry; only where it is larger are its elements looked at.
+// The first step's k-th largest thread maximum is a bound that the list's last entry cannot fall below, so few
+// elements ever enter a list; warps of a row share the highest such bound.
+template <typename T, int NW>
+__global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 8 : 4) k_token_logprobs(const LogprobArgs p) {
+    TB_GRID_DEP_ENTRY();
+    constexpr int E = 16 / sizeof(T), U = 4;
+    __shared__ unsigned long long keys[NW == 1 ? 1 : NW][32];
+    __shared__ Sums wsums[NW];
+    __shared__ unsigned long long shared_bound;
+    __shared__ int last;
+
+    const int lane = threadIdx.x & 31, warp = NW == 1 ? 0 : threadIdx.x >> 5;
+    const int64_t unit = NW == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
+    const int64_t row = NW == 1 ? unit : unit / p.splits;
+    if (NW == 1 && row >= p.rows) return;
+    const int split = NW == 1 ? 0 : (int)(unit - row * p.splits);
+    const T* x = static_cast<const T*>(p.logits) + row * p.stride;
+    const Row<T> r(x, p.vocab);
+    const int chunks = r.chunks(), per = NW == 1 ? chunks : (int)(((int64_t)chunks + p.splits - 1) / p.splits);
+    const int begin = split * per, stop = min(chunks, begin + per);
+    const float c = __fmul_rn(LOG2E, p.inv_t), margin = __fdiv_rn(40.f, c);
+    float given = 0.f;
+    if (p.logprob && warp == 0) {
+        const int64_t t = p.tokens[row];
+        if (t >= 0 && t < p.vocab) given = Elem<T>::get(x[t]);
+    }
+
+    float ref = -INFINITY, rmax = -INFINITY;
+    F2 z = {0.f, 0.f}, s = {0.f, 0.f};
+    int bad = 0;
+    unsigned long long list = 0, bound = 0;  // bound: keys below it are not among the row's `top` best
+    bool first = true;
+    for (int v0 = begin + warp * 32; first || v0 - warp * 32 < stop; v0 += NW * 32 * U) {
+        uint4 raw[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) raw[u] = r.load(v0 + u * NW * 32 + lane, stop);
+        float um[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) um[u] = Chunk<T>::vmax(raw[u]);
+        const float m = max_nan(max_nan(um[0], um[1]), max_nan(um[2], um[3]));
+        rmax = fmaxf(rmax, m);
+        float limit = INFINITY;
+        if (p.top) {
+            if (first) {
+                uint32_t o = sort32(ordered(m), lane);
+                if constexpr (NW > 1) {
+                    uint32_t (*buf)[32] = reinterpret_cast<uint32_t (*)[32]>(keys);
+                    o = merge_warps<NW>(o, buf, warp, lane);
+                    if (warp == 0) {
+                        o = __shfl_sync(0xffffffffu, o, p.top - 1);
+                        if (lane == 0) shared_bound = unordered(o) > -INFINITY ? (unsigned long long)o << 32 : 0;
+                    }
+                    __syncthreads();
+                } else {
+                    o = __shfl_sync(0xffffffffu, o, p.top - 1);
+                    bound = unordered(o) > -INFINITY ? (unsigned long long)o << 32 : 0;
+                }
+            }
+            if constexpr (NW > 1) {
+                const unsigned long long b = *(volatile unsigned long long*)&shared_bound;
+                bound = b > bound ? b : bound;
+            }
+            // a bound's own value can still come in, at a lower column, unless that column is behind this step
+            uint32_t o = (uint32_t)(bound >> 32);
+            const int64_t col0 = (int64_t)v0 * E - r.head;
+            if (bound && !((int64_t)key_col(bound) < col0)) o = o == 0x80000000u ? 0x7ffffffeu : o - 1;  // below 0 comes -0
+            limit = bound ? unordered(o) : -INFINITY;
+        }
+        first = false;
+        if (__any_sync(0xffffffffu, !(m <= fminf(limit, __fadd_rn(ref, margin))))) {
+            bad |= !(m < INFINITY);
+            if (m > __fadd_rn(ref, margin)) {
+                const float d = fmaxf(__fmul_rn(__fsub_rn(ref, m), c), EXP_FLOOR), f = exp2_fast(d);
+                s = {__fmul_rn(fmaf(z.x, d, s.x), f), __fmul_rn(fmaf(z.y, d, s.y), f)};
+                z = {__fmul_rn(z.x, f), __fmul_rn(z.y, f)};
+                ref = m;
+            }
+            if (p.top) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (!__any_sync(0xffffffffu, um[u] > limit)) continue;
+                    F2 f[E / 2];
+                    Chunk<T>::get(raw[u], f);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const float val = e & 1 ? f[e / 2].y : f[e / 2].x;
+                        unsigned some = __ballot_sync(0xffffffffu, val > limit);
+                        while (some) {
+                            const int from = __ffs((int)some) - 1;
+                            some &= some - 1;
+                            const int64_t col = (int64_t)(v0 + u * NW * 32 + from) * E + e - r.head;
+                            const unsigned long long key = top_key(__shfl_sync(0xffffffffu, val, from), (uint32_t)col);
+                            if (key > bound) {
+                                list = insert(list, key, lane);
+                                const unsigned long long k = __shfl_sync(0xffffffffu, list, p.top - 1);
+                                bound = k > bound ? k : bound;
+                            }
+                        }
+                    }
+                }
+                if (NW > 1 && lane == 0) atomicMax(&shared_bound, bound);
+            }
+        }
+        const F2 nref = {-ref, -ref}, cc = {c, c};
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            F2 f[E / 2];
+            Chunk<T>::get(raw[u], f);
+#pragma unroll
+            for (int e = 0; e < E / 2; ++e) {
+                F2 t = mul2(add2(f[e], nref), cc);
+                t = {fmaxf(t.x, EXP_FLOOR), fmaxf(t.y, EXP_FLOOR)};
+                const F2 q = {exp2_fast(t.x), exp2_fast(t.y)};
+                z = add2(z, q);
+                s = fma2(q, t, s);
+            }
+        }
+    }
+    // against the thread's true maximum, then the warp's
+    Sums a = {rmax, 0.f, 0.f, bad};
+    {
+        const float d = fmaxf(__fmul_rn(__fsub_rn(ref, rmax), c), EXP_FLOOR), f = exp2_fast(d);
+        const float zz = __fadd_rn(z.x, z.y), ss = __fadd_rn(s.x, s.y);
+        a.z = __fmul_rn(zz, f);
+        a.s = __fmul_rn(fmaf(zz, d, ss), f);
+    }
+    a = join_warp(a, c);
+    if constexpr (NW == 1) {
+        write_row<T>(p, row, a, lane < p.top ? list : 0, given, lane);
+    } else {
+        if (lane == 0) wsums[warp] = a;
+        __syncthreads();
+        if (p.top) list = merge_warps<NW>(lane < p.top ? list : 0ull, keys, warp, lane);
+        if (warp == 0) a = join_warp(lane < NW ? wsums[lane] : Sums{-INFINITY, 0.f, 0.f, 0}, c);
+        if (p.splits > 1) {
+            Part* part = p.parts + row * p.splits;
+            if (warp == 0) {
+                if (lane == 0) part[split].sums = a;
+                part[split].keys[lane] = list;
+                __threadfence();
+                __syncwarp();
+                if (lane == 0) {
+                    last = atomicAdd(&p.counters[row], 1) == p.splits - 1;
+                    if (last) p.counters[row] = 0;  // ready for the next launch
+                }
+            }
+            __syncthreads();
+            if (!last) return;
+            __threadfence();
+            a = {-INFINITY, 0.f, 0.f, 0};
+            list = 0;
+            for (int i = warp; i < p.splits; i += NW) {
+                a = join(a, {__ldcg(&part[i].sums.max), __ldcg(&part[i].sums.z), __ldcg(&part[i].sums.s), __ldcg(&part[i].sums.bad)}, c);
+                if (p.top) list = merge32(list, __ldcg(&part[i].keys[lane]), lane);
+            }
+            if (lane == 0) wsums[warp] = a;
+            __syncthreads();
+            if (p.top) list = merge_warps<NW>(list, keys, warp, lane);
+            if (warp == 0) a = join_warp(lane < NW ? wsums[lane] : Sums{-INFINITY, 0.f, 0.f, 0}, c);
+        }
+        if (warp == 0) write_row<T>(p, row, a, list, given, lane);
+    }
+}
+
+constexpr int LP_WARPS = 8;
+
+template <typename T> int launch_logprobs(tb_ctx* ctx, LogprobArgs p) {
+    constexpr int E = 16 / sizeof(T);
+    const int64_t chunks = ceil_div(p.vocab, E) + 1;
+    // a warp per row while a row is at most a step of it or rows are plenty for their length: @@W@@
+    if (chunks <= 32 * 4 + 1)
+        return launch(ctx, "k_token_logprobs", k_token_logprobs<T, 1>, dim3((unsigned)ceil_div(p.rows, 4)), dim3(128), 0, p);
+    // parts of a row of a step each at least, while the CTAs do not fill the GPU four times over
+    const int64_t steps = ceil_div(chunks, LP_WARPS * 32 * 4);
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({steps, 4 * ctx->sm_count / p.rows, 256}));
+    if (p.rows * p.splits > 2147483647) return fail(TB_ERR_UNSUPPORTED, "token logprobs: too many rows");
+    if (p.splits > 1) {
+        const int r = ensure_workspace(ctx, (size_t)(p.rows * p.splits) * sizeof(Part));
+        if (r != TB_OK) return r;
+        p.parts = static_cast<Part*>(ctx->ws);
+        p.counters = ctx->tile_cnt;  // rows < 4 per SM here
+    }
+    return launch(ctx, "k_token_logprobs", k_token_logprobs<T, LP_WARPS>, dim3((unsigned)(p.rows * p.splits)), dim3(LP_WARPS * 32), 0, p);
+}
+
+// ---- gradient ---------------------------------------------------------------------------------------
 struct LogprobBwdArgs {
     int64_t rows, vocab;
     const void* logits;
@@ -119,32 +497,87 @@ struct LogprobBwdArgs {
     const float* g_entropy;
     void* dlogits;
     int64_t d_stride;
+    int64_t parts;  // CTAs per row
 };
 
-template <typename T> __global__ void __launch_bounds__(256) k_token_logprobs_bwd(const LogprobBwdArgs p) {
+// d = (a (delta - p) - b p (log p + h)) / T, log p = (l - max) / T - log_sum, as
+// delta a / T - p (b / T log p + (a + b h) / T). A CTA takes 4 x 256 chunks of a row, or (WARP) each
+// of its warps a row of up to 4 x 32. In place is safe: a thread writes the chunks that it has read.
+template <typename T, bool WARP> __global__ void __launch_bounds__(256) k_token_logprobs_bwd(const LogprobBwdArgs p) {
     TB_GRID_DEP_ENTRY();
-    const int64_t row = blockIdx.x;
+    constexpr int E = 16 / sizeof(T), U = 4, NT = WARP ? 32 : 256;
+    const int64_t row = WARP ? (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5) : (int64_t)blockIdx.x / p.parts;
+    if (row >= p.rows) return;
+    const int part = WARP ? 0 : (int)((int64_t)blockIdx.x - row * p.parts);
+    const int tid = WARP ? threadIdx.x & 31 : threadIdx.x;
     const T* x = static_cast<const T*>(p.logits) + row * p.stride;
     T* d = static_cast<T*>(p.dlogits) + row * p.d_stride;
+    const Row<T> r(x, p.vocab);
+    const int stop = r.chunks(), v0 = part * NT * U + tid;
+    uint4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u] = r.load(v0 + u * NT, stop);
+
     const float m = p.row_max[row], logz = p.log_sum[row];
-    int64_t tok = p.g_logprob && p.tokens ? p.tokens[row] : -1;
+    const int64_t tok = p.g_logprob && p.tokens ? p.tokens[row] : -1;
     const float a = tok >= 0 ? p.g_logprob[row] : 0.f, b = p.g_entropy ? p.g_entropy[row] : 0.f;
     const float h = p.g_entropy ? p.entropy[row] : 0.f;
     const bool empty = m == -INFINITY, bad = logz != logz || tok >= p.vocab;
-    for (int64_t i = threadIdx.x; i < p.vocab; i += blockDim.x) {
-        float g = nan_f();
-        if (empty) g = 0.f;
-        else if (!bad) {
-            const float lp = fmaxf(__fsub_rn(__fmul_rn(__fsub_rn(Elem<T>::get(x[i]), m), p.inv_t), logz), -200.f);
-            const float q = expf(lp);
-            g = __fmul_rn(__fsub_rn(i == tok ? a : 0.f, __fmul_rn(q, fmaf(b, __fadd_rn(lp, h), a))), p.inv_t);
+    const float at = __fmul_rn(a, p.inv_t), bt = __fmul_rn(b, p.inv_t), ct = __fmul_rn(fmaf(b, h, a), p.inv_t);
+    const F2 nm = {-m, -m}, it = {p.inv_t, p.inv_t}, nz = {-logz, -logz}, b2 = {bt, bt}, c2 = {ct, ct}, l2 = {LOG2E, LOG2E};
+    const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int v = v0 + u * NT;
+        if (v >= stop) continue;
+        F2 f[E / 2];
+        Chunk<T>::get(raw[u], f);
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e) {
+            F2 lp = fma2(add2(f[e], nm), it, nz);
+            lp = {fmaxf(lp.x, EXP_FLOOR), fmaxf(lp.y, EXP_FLOOR)};
+            const F2 t = mul2(lp, l2);
+            const F2 q = {-exp2_fast(t.x), -exp2_fast(t.y)};
+            f[e] = mul2(q, fma2(b2, lp, c2));
         }
-        d[i] = Elem<T>::put(g);
+        const int64_t i0 = (int64_t)v * E - r.head;
+        if (tok >= i0 && tok < i0 + E) {
+#pragma unroll
+            for (int e = 0; e < E / 2; ++e) {
+                if (tok == i0 + 2 * e) f[e].x = __fadd_rn(f[e].x, at);
+                if (tok == i0 + 2 * e + 1) f[e].y = __fadd_rn(f[e].y, at);
+            }
+        }
+        if (empty || bad) {
+            const float fill = bad ? nan_f() : 0.f;
+#pragma unroll
+            for (int e = 0; e < E / 2; ++e) f[e] = {fill, fill};
+        }
+        const uint4 out = Chunk<T>::put(f);
+        if (same && r.whole(v)) {
+            *reinterpret_cast<uint4*>(d + i0) = out;
+        } else {
+            T t[E];
+            memcpy(t, &out, 16);
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (i0 + e >= 0 && i0 + e < p.vocab) d[i0 + e] = t[e];
+        }
     }
 }
 
+template <typename T> int launch_bwd(tb_ctx* ctx, LogprobBwdArgs p) {
+    constexpr int E = 16 / sizeof(T);
+    const int64_t chunks = ceil_div(p.vocab, E) + 1;  // one more where a row starts inside a chunk
+    if (chunks <= 32 * 4)
+        return launch(ctx, "k_token_logprobs_bwd", k_token_logprobs_bwd<T, true>, dim3((unsigned)ceil_div(p.rows, 8)), dim3(256), 0, p);
+    p.parts = ceil_div(chunks, 256 * 4);
+    if (p.rows * p.parts > 2147483647) return fail(TB_ERR_UNSUPPORTED, "token logprobs: more than 2^31 parts of rows");
+    return launch(ctx, "k_token_logprobs_bwd", k_token_logprobs_bwd<T, false>, dim3((unsigned)(p.rows * p.parts)), dim3(256), 0, p);
+}
+
 int check_logits(int64_t rows, int64_t vocab, const void* logits, int64_t type, int64_t stride, float temperature) {
-    if (rows < 0 || vocab <= 0 || rows > 2147483647 || vocab > 2147483647) return fail(TB_ERR_INVALID, "token logprobs: bad shape");
+    if (rows < 0 || vocab <= 0 || rows > 2147483647 || vocab > 2147483000) return fail(TB_ERR_INVALID, "token logprobs: bad shape");
     if (!elem_type_ok(type)) return fail(TB_ERR_UNSUPPORTED, "token logprobs: element type %lld", (long long)type);
     if (!(temperature >= 0x1p-100f && temperature <= 0x1p100f)) return fail(TB_ERR_INVALID, "token logprobs: temperature has to be positive and finite");
     if (rows > 1 && stride < vocab) return fail(TB_ERR_INVALID, "token logprobs: row stride below the row's length");
@@ -171,10 +604,8 @@ int tb_token_logprobs_fwd(tb_ctx* ctx, int64_t rows, int64_t vocab, const void* 
     if (top > TOP_MAX) return fail(TB_ERR_UNSUPPORTED, "token logprobs: top over %d", TOP_MAX);
     if (rows == 0) return TB_OK;
     if ((tokens && !logprob) || (top && (!top_logprob || !top_token))) return fail(TB_ERR_INVALID, "token logprobs: null pointer");
-    const LogprobArgs p{rows, vocab, logits, stride, tokens, 1.f / temperature, (int)top, tokens ? logprob : nullptr, entropy, lse, row_max, log_sum, top_logprob, top_token};
-    return elem_dispatch(type, [&](auto t) {
-        return launch(ctx, "k_token_logprobs", k_token_logprobs<decltype(t)>, dim3((unsigned)rows), dim3(256), 0, p);
-    });
+    LogprobArgs p{rows, vocab, logits, stride, tokens, 1.f / temperature, (int)top, tokens ? logprob : nullptr, entropy, lse, row_max, log_sum, top_logprob, top_token, 1, nullptr, nullptr};
+    return elem_dispatch(type, [&](auto t) { return launch_logprobs<decltype(t)>(ctx, p); });
 }
 
 int tb_token_logprobs_bwd(tb_ctx* ctx, int64_t rows, int64_t vocab, const void* logits, int64_t type,
@@ -189,10 +620,8 @@ int tb_token_logprobs_bwd(tb_ctx* ctx, int64_t rows, int64_t vocab, const void* 
     if (!row_max || !log_sum || !dlogits || (g_logprob && !tokens) || (g_entropy && !entropy)) return fail(TB_ERR_INVALID, "token logprobs: null pointer");
     if ((uintptr_t)dlogits % elem_size(type)) return fail(TB_ERR_INVALID, "token logprobs: misaligned pointer");
     if (dlogits == logits && rows > 1 && d_stride != stride) return fail(TB_ERR_INVALID, "token logprobs: in place with another row stride");
-    const LogprobBwdArgs p{rows, vocab, logits, stride, tokens, 1.f / temperature, row_max, log_sum, entropy, g_logprob, g_entropy, dlogits, d_stride};
-    return elem_dispatch(type, [&](auto t) {
-        return launch(ctx, "k_token_logprobs_bwd", k_token_logprobs_bwd<decltype(t)>, dim3((unsigned)rows), dim3(256), 0, p);
-    });
+    const LogprobBwdArgs p{rows, vocab, logits, stride, tokens, 1.f / temperature, row_max, log_sum, entropy, g_logprob, g_entropy, dlogits, d_stride, 1};
+    return elem_dispatch(type, [&](auto t) { return launch_bwd<decltype(t)>(ctx, p); });
 }
 
 }  // extern "C"
