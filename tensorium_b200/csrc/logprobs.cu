@@ -291,196 +291,249 @@ __device__ __forceinline__ void write_row(const LogprobArgs& p, int64_t row, con
     }
 }
 
-// One pass over the logits. NW warps work on a row (1: a warp has a row to itself, four in a CTA), or
-// on one of `splits` parts of a row where the rows alone do not fill the GPU.
-//
-// Sums: each thread keeps sum 2^t and sum t 2^t against a reference of its own, an earlier logit,
-// and moves the reference only when a logit is 2^40 above it; the sums are floating point, so nothing is
-// lost below that, and most steps need no new maximum. Alternatives: a step's largest logit per thread
-// is compared with the list's last entry; only where it is larger are its elements looked at.
-// The first step's k-th largest thread maximum is a bound that the list's last entry cannot fall below, so few
-// elements ever enter a list; warps of a row share the highest such bound.
-template <typename T, int NW>
-__global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 8 : 4) k_token_logprobs(const LogprobArgs p) {
-    TB_GRID_DEP_ENTRY();
-    constexpr int E = 16 / sizeof(T), U = 4;
-    __shared__ unsigned long long keys[NW == 1 ? 1 : NW][32];
-    __shared__ Sums wsums[NW];
-    __shared__ unsigned long long shared_bound;
-    __shared__ int last;
-
-    const int lane = threadIdx.x & 31, warp = NW == 1 ? 0 : threadIdx.x >> 5;
-    const int64_t unit = NW == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
-    const int64_t row = NW == 1 ? unit : unit / p.splits;
-    if (NW == 1 && row >= p.rows) return;
-    const int split = NW == 1 ? 0 : (int)(unit - row * p.splits);
-    const T* x = static_cast<const T*>(p.logits) + row * p.stride;
-    const Row<T> r(x, p.vocab);
-    const int chunks = r.chunks(), per = NW == 1 ? chunks : (int)(((int64_t)chunks + p.splits - 1) / p.splits);
-    const int begin = split * per, stop = min(chunks, begin + per);
-    const float c = __fmul_rn(LOG2E, p.inv_t), margin = __fdiv_rn(40.f, c);
-    float given = 0.f;
-    if (p.logprob && warp == 0) {
-        const int64_t t = p.tokens[row];
-        if (t >= 0 && t < p.vocab) given = Elem<T>::get(x[t]);
-    }
-
-    float ref = -INFINITY, rmax = -INFINITY;
+// The sums of one thread: against a reference of its own, an earlier logit, moved only when a logit is
+// 2^40 above it. The sums are floating point, so nothing is lost below that, and most steps need no new
+// maximum.
+struct Running {
+    float ref = -INFINITY, max = -INFINITY;
     F2 z = {0.f, 0.f}, s = {0.f, 0.f};
     int bad = 0;
-    unsigned long long list = 0, bound = 0;  // bound: keys below it are not among the row's `top` best
-    bool first = true;
-    for (int v0 = begin + warp * 32; first || v0 - warp * 32 < stop; v0 += NW * 32 * U) {
+    // before logits up to m (NaN: one of them is) are added
+    __device__ __forceinline__ void raise(float m, float c, float margin) {
+        max = fmaxf(max, m);
+        if (!(m <= __fadd_rn(ref, margin))) {
+            bad |= !(m < INFINITY);
+            const float d = fmaxf(__fmul_rn(__fsub_rn(ref, m), c), EXP_FLOOR), f = exp2_fast(d);
+            s = {__fmul_rn(fmaf(z.x, d, s.x), f), __fmul_rn(fmaf(z.y, d, s.y), f)};
+            z = {__fmul_rn(z.x, f), __fmul_rn(z.y, f)};
+            ref = fmaxf(ref, m);
+        }
+    }
+    template <typename T> __device__ __forceinline__ void add(const uint4& raw, float c) {
+        constexpr int E = 16 / sizeof(T);
+        F2 f[E / 2];
+        Chunk<T>::get(raw, f);
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e) {
+            F2 t = mul2(add2(f[e], {-ref, -ref}), {c, c});
+            t = {fmaxf(t.x, EXP_FLOOR), fmaxf(t.y, EXP_FLOOR)};
+            const F2 q = {exp2_fast(t.x), exp2_fast(t.y)};
+            z = add2(z, q);
+            s = fma2(q, t, s);
+        }
+    }
+    // against the thread's true maximum
+    __device__ __forceinline__ Sums sums(float c) const {
+        const float d = fmaxf(__fmul_rn(__fsub_rn(ref, max), c), EXP_FLOOR), f = exp2_fast(d);
+        const float zz = __fadd_rn(z.x, z.y), ss = __fadd_rn(s.x, s.y);
+        return {max, __fmul_rn(zz, f), __fmul_rn(fmaf(zz, d, ss), f), bad};
+    }
+};
+
+template <typename T> __device__ __forceinline__ float given_logit(const LogprobArgs& p, int64_t row, const T* x) {
+    if (!p.logprob) return 0.f;
+    const int64_t t = p.tokens[row];
+    return t >= 0 && t < p.vocab ? Elem<T>::get(x[t]) : 0.f;
+}
+
+// The largest float below the value of a bound's key, so that `logit > limit_of(bound)` lets in equal logits
+// at lower columns; -infinity for no bound.
+__device__ __forceinline__ float limit_of(unsigned long long bound) {
+    const uint32_t o = (uint32_t)(bound >> 32);
+    return !bound ? -INFINITY : unordered(o == 0x80000000u ? 0x7ffffffeu : o - 1);  // below 0 comes -0
+}
+
+// Into a warp's list: the keys (0: none) of 32 lanes that are above the bound.
+__device__ __forceinline__ void take(unsigned long long& list, unsigned long long& bound, unsigned long long key, int top, int lane) {
+    unsigned some = __ballot_sync(0xffffffffu, key > bound);
+    if (__popc(some) > 6) {  // six insertions cost what a sort of the 32 does
+        list = merge32(list, sort32(key > bound ? key : 0ull, lane), lane);
+        some = 0;
+    }
+    while (some) {
+        const unsigned long long k = __shfl_sync(0xffffffffu, key, __ffs((int)some) - 1);
+        some &= some - 1;
+        list = insert(list, k, lane);
+    }
+    const unsigned long long k = __shfl_sync(0xffffffffu, list, top - 1);
+    bound = k > bound ? k : bound;
+}
+
+// A row to a warp, four to a CTA: rows of up to 512 bytes a lane. The k-th largest of the lanes' maxima is
+// a bound that the k-th best cannot fall below, so few logits are looked at again, from the registers.
+template <typename T> __global__ void __launch_bounds__(128, 8) k_token_logprobs_warp(const LogprobArgs p) {
+    TB_GRID_DEP_ENTRY();
+    constexpr int E = 16 / sizeof(T), U = 4;
+    const int lane = threadIdx.x & 31;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (row >= p.rows) return;
+    const T* x = static_cast<const T*>(p.logits) + row * p.stride;
+    const Row<T> r(x, p.vocab);
+    const int stop = r.chunks();
+    const float c = __fmul_rn(LOG2E, p.inv_t), margin = __fdiv_rn(40.f, c);
+    const float given = given_logit(p, row, x);
+
+    Running a;
+    unsigned long long list = 0, bound = 0;  // bound: keys up to it are not among the `top` best
+    for (int v0 = 0; v0 < stop; v0 += 32 * U) {
         uint4 raw[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) raw[u] = r.load(v0 + u * NW * 32 + lane, stop);
+        for (int u = 0; u < U; ++u) raw[u] = r.load(v0 + u * 32 + lane, stop);
         float um[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) um[u] = Chunk<T>::vmax(raw[u]);
         const float m = max_nan(max_nan(um[0], um[1]), max_nan(um[2], um[3]));
-        rmax = fmaxf(rmax, m);
-        float limit = INFINITY;
-        if (p.top) {
-            if (first) {
-                uint32_t o = sort32(ordered(m), lane);
-                if constexpr (NW > 1) {
-                    uint32_t (*buf)[32] = reinterpret_cast<uint32_t (*)[32]>(keys);
-                    o = merge_warps<NW>(o, buf, warp, lane);
-                    if (warp == 0) {
-                        o = __shfl_sync(0xffffffffu, o, p.top - 1);
-                        if (lane == 0) shared_bound = unordered(o) > -INFINITY ? (unsigned long long)o << 32 : 0;
-                    }
-                    __syncthreads();
-                } else {
-                    o = __shfl_sync(0xffffffffu, o, p.top - 1);
-                    bound = unordered(o) > -INFINITY ? (unsigned long long)o << 32 : 0;
-                }
-            }
-            if constexpr (NW > 1) {
-                const unsigned long long b = *(volatile unsigned long long*)&shared_bound;
-                bound = b > bound ? b : bound;
-            }
-            // a bound's own value can still come in, at a lower column, unless that column is behind this step
-            uint32_t o = (uint32_t)(bound >> 32);
-            const int64_t col0 = (int64_t)v0 * E - r.head;
-            if (bound && !((int64_t)key_col(bound) < col0)) o = o == 0x80000000u ? 0x7ffffffeu : o - 1;  // below 0 comes -0
-            limit = bound ? unordered(o) : -INFINITY;
-        }
-        first = false;
-        if (__any_sync(0xffffffffu, !(m <= fminf(limit, __fadd_rn(ref, margin))))) {
-            bad |= !(m < INFINITY);
-            if (m > __fadd_rn(ref, margin)) {
-                const float d = fmaxf(__fmul_rn(__fsub_rn(ref, m), c), EXP_FLOOR), f = exp2_fast(d);
-                s = {__fmul_rn(fmaf(z.x, d, s.x), f), __fmul_rn(fmaf(z.y, d, s.y), f)};
-                z = {__fmul_rn(z.x, f), __fmul_rn(z.y, f)};
-                ref = m;
-            }
-            if (p.top) {
+        a.raise(m, c, margin);
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    if (!__any_sync(0xffffffffu, um[u] > limit)) continue;
-                    F2 f[E / 2];
-                    Chunk<T>::get(raw[u], f);
-#pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        const float val = e & 1 ? f[e / 2].y : f[e / 2].x;
-                        unsigned some = __ballot_sync(0xffffffffu, val > limit);
-                        while (some) {
-                            const int from = __ffs((int)some) - 1;
-                            some &= some - 1;
-                            const int64_t col = (int64_t)(v0 + u * NW * 32 + from) * E + e - r.head;
-                            const unsigned long long key = top_key(__shfl_sync(0xffffffffu, val, from), (uint32_t)col);
-                            if (key > bound) {
-                                list = insert(list, key, lane);
-                                const unsigned long long k = __shfl_sync(0xffffffffu, list, p.top - 1);
-                                bound = k > bound ? k : bound;
-                            }
-                        }
-                    }
-                }
-                if (NW > 1 && lane == 0) atomicMax(&shared_bound, bound);
-            }
+        for (int u = 0; u < U; ++u) a.add<T>(raw[u], c);
+        if (!p.top) continue;
+        if (v0 == 0) {
+            const uint32_t o = __shfl_sync(0xffffffffu, sort32(ordered(m), lane), p.top - 1);
+            if (unordered(o) > -INFINITY) bound = (unsigned long long)o << 32;
         }
-        const F2 nref = {-ref, -ref}, cc = {c, c};
 #pragma unroll
         for (int u = 0; u < U; ++u) {
+            if (!__any_sync(0xffffffffu, um[u] > limit_of(bound))) continue;
             F2 f[E / 2];
             Chunk<T>::get(raw[u], f);
 #pragma unroll
-            for (int e = 0; e < E / 2; ++e) {
-                F2 t = mul2(add2(f[e], nref), cc);
-                t = {fmaxf(t.x, EXP_FLOOR), fmaxf(t.y, EXP_FLOOR)};
-                const F2 q = {exp2_fast(t.x), exp2_fast(t.y)};
-                z = add2(z, q);
-                s = fma2(q, t, s);
+            for (int e = 0; e < E; ++e) {
+                const float v = e & 1 ? f[e / 2].y : f[e / 2].x;
+                const bool in = v > limit_of(bound);
+                if (__any_sync(0xffffffffu, in))
+                    take(list, bound, in ? top_key(v, (uint32_t)((v0 + u * 32 + lane) * E + e - r.head)) : 0ull, p.top, lane);
             }
         }
     }
-    // against the thread's true maximum, then the warp's
-    Sums a = {rmax, 0.f, 0.f, bad};
-    {
-        const float d = fmaxf(__fmul_rn(__fsub_rn(ref, rmax), c), EXP_FLOOR), f = exp2_fast(d);
-        const float zz = __fadd_rn(z.x, z.y), ss = __fadd_rn(s.x, s.y);
-        a.z = __fmul_rn(zz, f);
-        a.s = __fmul_rn(fmaf(zz, d, ss), f);
-    }
-    a = join_warp(a, c);
-    if constexpr (NW == 1) {
-        write_row<T>(p, row, a, lane < p.top ? list : 0, given, lane);
-    } else {
-        if (lane == 0) wsums[warp] = a;
-        __syncthreads();
-        if (p.top) list = merge_warps<NW>(lane < p.top ? list : 0ull, keys, warp, lane);
-        if (warp == 0) a = join_warp(lane < NW ? wsums[lane] : Sums{-INFINITY, 0.f, 0.f, 0}, c);
-        if (p.splits > 1) {
-            Part* part = p.parts + row * p.splits;
-            if (warp == 0) {
-                if (lane == 0) part[split].sums = a;
-                part[split].keys[lane] = list;
-                __threadfence();
-                __syncwarp();
-                if (lane == 0) {
-                    last = atomicAdd(&p.counters[row], 1) == p.splits - 1;
-                    if (last) p.counters[row] = 0;  // ready for the next launch
-                }
-            }
-            __syncthreads();
-            if (!last) return;
-            __threadfence();
-            a = {-INFINITY, 0.f, 0.f, 0};
-            list = 0;
-            for (int i = warp; i < p.splits; i += NW) {
-                a = join(a, {__ldcg(&part[i].sums.max), __ldcg(&part[i].sums.z), __ldcg(&part[i].sums.s), __ldcg(&part[i].sums.bad)}, c);
-                if (p.top) list = merge32(list, __ldcg(&part[i].keys[lane]), lane);
-            }
-            if (lane == 0) wsums[warp] = a;
-            __syncthreads();
-            if (p.top) list = merge_warps<NW>(list, keys, warp, lane);
-            if (warp == 0) a = join_warp(lane < NW ? wsums[lane] : Sums{-INFINITY, 0.f, 0.f, 0}, c);
-        }
-        if (warp == 0) write_row<T>(p, row, a, list, given, lane);
-    }
+    write_row<T>(p, row, join_warp(a.sums(c), c), lane < p.top ? list : 0, given, lane);
 }
 
-constexpr int LP_WARPS = 8;
+// A row, or one of `splits` parts of it, to a CTA. Each step of a thread is a group of U chunks; the groups'
+// maxima stay in shared memory, so that after the one pass only the groups that can hold one of
+// the best are read again: those whose maximum reaches the k-th largest of the threads' maxima, about k of them.
+constexpr int LP_WARPS = 8, LP_U = 4;
+template <typename T> constexpr int LP_STEPS = sizeof(T) == 4 ? 16 : 32;  // most steps of a part
+
+template <typename T> __global__ void __launch_bounds__(LP_WARPS * 32, 4) k_token_logprobs(const LogprobArgs p) {
+    TB_GRID_DEP_ENTRY();
+    constexpr int E = 16 / sizeof(T), U = LP_U, NT = LP_WARPS * 32;
+    __shared__ T group_max[LP_STEPS<T>][NT];
+    __shared__ uint16_t queue[LP_STEPS<T> * NT];
+    __shared__ unsigned long long keys[LP_WARPS][32];
+    __shared__ Sums wsums[LP_WARPS];
+    __shared__ unsigned long long shared_bound;
+    __shared__ int queued, last;
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t row = (int64_t)blockIdx.x / p.splits;
+    const int split = (int)((int64_t)blockIdx.x - row * p.splits);
+    const T* x = static_cast<const T*>(p.logits) + row * p.stride;
+    const Row<T> r(x, p.vocab);
+    const int chunks = r.chunks(), per = (int)(((int64_t)chunks + p.splits - 1) / p.splits);
+    const int begin = (int)min((int64_t)chunks, (int64_t)split * per), stop = min(chunks, begin + per);
+    const float c = __fmul_rn(LOG2E, p.inv_t), margin = __fdiv_rn(40.f, c);
+    const float given = warp == 0 ? given_logit(p, row, x) : 0.f;
+    if (tid == 0) queued = 0;
+
+    Running a;
+    int steps = 0;
+    for (int v0 = begin; v0 < stop; v0 += NT * U, ++steps) {
+        uint4 raw[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) raw[u] = r.load(v0 + u * NT + tid, stop);
+        float m = Chunk<T>::vmax(raw[0]);
+#pragma unroll
+        for (int u = 1; u < U; ++u) m = max_nan(m, Chunk<T>::vmax(raw[u]));
+        if (p.top) group_max[steps][tid] = Elem<T>::put(m);  // exact: m is one of the logits
+        a.raise(m, c, margin);
+#pragma unroll
+        for (int u = 0; u < U; ++u) a.add<T>(raw[u], c);
+    }
+    Sums w = join_warp(a.sums(c), c);
+    if (lane == 0) wsums[warp] = w;
+    unsigned long long list = 0;
+    if (p.top) {
+        uint32_t o = merge_warps<LP_WARPS>(sort32(ordered(a.max), lane), reinterpret_cast<uint32_t (*)[32]>(keys), warp, lane);
+        if (warp == 0) {
+            o = __shfl_sync(0xffffffffu, o, p.top - 1);
+            if (lane == 0) shared_bound = unordered(o) > -INFINITY ? (unsigned long long)o << 32 : 0;
+        }
+        __syncthreads();
+        unsigned long long bound = shared_bound;
+        const float limit = limit_of(bound);
+        for (int i = 0; i < steps; ++i)
+            if (Elem<T>::get(group_max[i][tid]) > limit) queue[atomicAdd(&queued, 1)] = (uint16_t)(i * NT + tid);
+        __syncthreads();
+        const int n = queued;
+        for (int q = warp; q < n; q += LP_WARPS) {
+            const int g = queue[q];
+            // an element a lane; every lane takes part in take(), also those past the group's U * E
+            static_assert(U * E <= 32, "a group is read by one warp at a time");
+            const int v = begin + (g / NT) * NT * U + (lane / E) * NT + g % NT;
+            const int64_t at = (int64_t)v * E + lane % E;
+            const bool in = lane < U * E && v < stop && at >= r.head && at < r.end;
+            const float l = in ? Elem<T>::get(r.base[at]) : -INFINITY;
+            take(list, bound, l > limit ? top_key(l, (uint32_t)(at - r.head)) : 0ull, p.top, lane);
+        }
+        list = merge_warps<LP_WARPS>(lane < p.top ? list : 0ull, keys, warp, lane);
+    } else {
+        __syncthreads();
+    }
+    if (warp == 0) w = join_warp(lane < LP_WARPS ? wsums[lane] : Sums{-INFINITY, 0.f, 0.f, 0}, c);
+    if (p.splits > 1) {
+        Part* part = p.parts + row * p.splits;
+        if (warp == 0) {
+            if (lane == 0) part[split].sums = w;
+            part[split].keys[lane] = list;
+            __threadfence();
+            __syncwarp();
+            if (lane == 0) {
+                last = atomicAdd(&p.counters[row], 1) == p.splits - 1;
+                if (last) p.counters[row] = 0;  // ready for the next launch
+            }
+        }
+        __syncthreads();
+        if (!last) return;
+        __threadfence();
+        w = {-INFINITY, 0.f, 0.f, 0};
+        list = 0;
+        for (int i = warp; i < p.splits; i += LP_WARPS) {
+            w = join(w, {__ldcg(&part[i].sums.max), __ldcg(&part[i].sums.z), __ldcg(&part[i].sums.s), __ldcg(&part[i].sums.bad)}, c);
+            if (p.top) list = merge32(list, __ldcg(&part[i].keys[lane]), lane);
+        }
+        if (lane == 0) wsums[warp] = w;
+        __syncthreads();
+        if (p.top) list = merge_warps<LP_WARPS>(list, keys, warp, lane);
+        if (warp == 0) w = join_warp(lane < LP_WARPS ? wsums[lane] : Sums{-INFINITY, 0.f, 0.f, 0}, c);
+    }
+    if (warp == 0) write_row<T>(p, row, w, list, given, lane);
+}
 
 template <typename T> int launch_logprobs(tb_ctx* ctx, LogprobArgs p) {
     constexpr int E = 16 / sizeof(T);
-    const int64_t chunks = ceil_div(p.vocab, E) + 1;
-    // a warp per row while a row is at most a step of it or rows are plenty for their length: @@W@@
+    const int64_t chunks = ceil_div(p.vocab, E) + 1;  // one more where a row starts inside a chunk
+    // a warp per row while a row is at most a step of it: @@W@@
     if (chunks <= 32 * 4 + 1)
-        return launch(ctx, "k_token_logprobs", k_token_logprobs<T, 1>, dim3((unsigned)ceil_div(p.rows, 4)), dim3(128), 0, p);
-    // parts of a row of a step each at least, while the CTAs do not fill the GPU four times over
-    const int64_t steps = ceil_div(chunks, LP_WARPS * 32 * 4);
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({steps, 4 * ctx->sm_count / p.rows, 256}));
+        return launch(ctx, "k_token_logprobs_warp", k_token_logprobs_warp<T>, dim3((unsigned)ceil_div(p.rows, 4)), dim3(128), 0, p);
+    // a row in parts of a step each at least while the CTAs do not fill the GPU four times over, and of LP_STEPS at
+    // most
+    const int64_t step = LP_WARPS * 32 * LP_U, steps = ceil_div(chunks, step);
+    p.splits = (int)std::max<int64_t>(std::min<int64_t>({steps, 4 * ctx->sm_count / p.rows, 256}), ceil_div(steps, LP_STEPS<T>));
     if (p.rows * p.splits > 2147483647) return fail(TB_ERR_UNSUPPORTED, "token logprobs: too many rows");
     if (p.splits > 1) {
-        const int r = ensure_workspace(ctx, (size_t)(p.rows * p.splits) * sizeof(Part));
+        // partial results and counters (zeroed: the context's own are too few for many long rows)
+        const size_t parts = (size_t)(p.rows * p.splits) * sizeof(Part);
+        const bool own = p.rows > ctx->tile_cnt_len;
+        const int r = ensure_workspace(ctx, parts + (own ? p.rows * sizeof(int) : 0));
         if (r != TB_OK) return r;
         p.parts = static_cast<Part*>(ctx->ws);
-        p.counters = ctx->tile_cnt;  // rows < 4 per SM here
+        p.counters = ctx->tile_cnt;
+        if (own) {
+            p.counters = reinterpret_cast<int*>(static_cast<char*>(ctx->ws) + parts);
+            TB_CHECK_CUDA(cudaMemsetAsync(p.counters, 0, p.rows * sizeof(int), ctx->stream));
+        }
     }
-    return launch(ctx, "k_token_logprobs", k_token_logprobs<T, LP_WARPS>, dim3((unsigned)(p.rows * p.splits)), dim3(LP_WARPS * 32), 0, p);
+    return launch(ctx, "k_token_logprobs", k_token_logprobs<T>, dim3((unsigned)(p.rows * p.splits)), dim3(LP_WARPS * 32), 0, p);
 }
 
 // ---- gradient ---------------------------------------------------------------------------------------
