@@ -98,8 +98,13 @@ constexpr float EXP_FLOOR = -200.f;
 template <typename T> struct Chunk;
 template <> struct Chunk<float> {
     static constexpr uint32_t MASKED = 0xff800000u;  // -infinity
-    static __device__ __forceinline__ float vmax(const uint4& r) {
-        return max_nan(max_nan(__uint_as_float(r.x), __uint_as_float(r.y)), max_nan(__uint_as_float(r.z), __uint_as_float(r.w)));
+    // the largest logit of n chunks, NaN if one is
+    template <int N> static __device__ __forceinline__ float vmax(const uint4 (&r)[N]) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            m = max_nan(m, max_nan(max_nan(__uint_as_float(r[i].x), __uint_as_float(r[i].y)), max_nan(__uint_as_float(r[i].z), __uint_as_float(r[i].w))));
+        return m;
     }
     static __device__ __forceinline__ void get(const uint4& r, F2* f) {
         f[0] = {__uint_as_float(r.x), __uint_as_float(r.y)};
@@ -111,10 +116,14 @@ template <> struct Chunk<float> {
 };
 template <> struct Chunk<__nv_bfloat16> {
     static constexpr uint32_t MASKED = 0xff80ff80u;
-    static __device__ __forceinline__ float vmax(const uint4& r) {
+    template <int N> static __device__ __forceinline__ float vmax(const uint4 (&r)[N]) {
         auto h = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
-        const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h(r.x), h(r.y)), __hmax2_nan(h(r.z), h(r.w)));
-        return max_nan(__low2float(m), __high2float(m));
+        __nv_bfloat162 m[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) m[i] = __hmax2_nan(__hmax2_nan(h(r[i].x), h(r[i].y)), __hmax2_nan(h(r[i].z), h(r[i].w)));
+#pragma unroll
+        for (int i = 1; i < N; ++i) m[0] = __hmax2_nan(m[0], m[i]);
+        return max_nan(__low2float(m[0]), __high2float(m[0]));
     }
     static __device__ __forceinline__ F2 two(uint32_t w) { return {__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)}; }
     static __device__ __forceinline__ void get(const uint4& r, F2* f) { f[0] = two(r.x), f[1] = two(r.y), f[2] = two(r.z), f[3] = two(r.w); }
@@ -126,10 +135,14 @@ template <> struct Chunk<__nv_bfloat16> {
 };
 template <> struct Chunk<__half> {
     static constexpr uint32_t MASKED = 0xfc00fc00u;
-    static __device__ __forceinline__ float vmax(const uint4& r) {
+    template <int N> static __device__ __forceinline__ float vmax(const uint4 (&r)[N]) {
         auto h = [](uint32_t w) { return *reinterpret_cast<const __half2*>(&w); };
-        const __half2 m = __hmax2_nan(__hmax2_nan(h(r.x), h(r.y)), __hmax2_nan(h(r.z), h(r.w)));
-        return max_nan(__low2float(m), __high2float(m));
+        __half2 m[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) m[i] = __hmax2_nan(__hmax2_nan(h(r[i].x), h(r[i].y)), __hmax2_nan(h(r[i].z), h(r[i].w)));
+#pragma unroll
+        for (int i = 1; i < N; ++i) m[0] = __hmax2_nan(m[0], m[i]);
+        return max_nan(__low2float(m[0]), __high2float(m[0]));
     }
     static __device__ __forceinline__ F2 two(uint32_t w) {
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
@@ -156,7 +169,7 @@ template <typename T> struct Row {
         end = head + (int)vocab;
     }
     __device__ __forceinline__ int chunks() const { return (int)(((int64_t)end + E - 1) / E); }
-    __device__ __forceinline__ bool whole(int v) const { return v * (int64_t)E >= head && (v + 1) * (int64_t)E <= end; }
+    __device__ __forceinline__ bool whole(int v) const { return v >= (head ? 1 : 0) && v < end / E; }
     __device__ __forceinline__ uint4 load(int v, int stop) const {
         if (v < stop && whole(v)) return *reinterpret_cast<const uint4*>(base + (int64_t)v * E);
         uint4 r = make_uint4(Chunk<T>::MASKED, Chunk<T>::MASKED, Chunk<T>::MASKED, Chunk<T>::MASKED);
@@ -171,6 +184,18 @@ template <typename T> struct Row {
             memcpy(&r, t, 16);
         }
         return r;
+    }
+    // chunks v0 + u * apart + at, u < N, of a step that begins at chunk v0 (the same for all its threads) and
+    // spans N * apart of them: most steps are whole and need no check for a chunk
+    template <int N> __device__ __forceinline__ void step(uint4 (&r)[N], int v0, int at, int apart, int stop) const {
+        if (whole(v0) && v0 + N * apart <= min(stop, end / E)) {
+            const uint4* q = reinterpret_cast<const uint4*>(base) + v0 + at;
+#pragma unroll
+            for (int u = 0; u < N; ++u) r[u] = q[u * apart];
+        } else {
+#pragma unroll
+            for (int u = 0; u < N; ++u) r[u] = load(v0 + u * apart + at, stop);
+        }
     }
 };
 
@@ -233,14 +258,16 @@ __device__ __forceinline__ Sums join(const Sums& a, const Sums& b, float c) {
     return r;
 }
 __device__ __forceinline__ Sums join_warp(Sums a, float c) {
+    const float max = unordered(__reduce_max_sync(0xffffffffu, ordered(a.max)));
+    const float d = fmaxf(__fmul_rn(__fsub_rn(a.max, max), c), EXP_FLOOR), f = exp2_fast(d);
+    a.s = __fmul_rn(fmaf(a.z, d, a.s), f);
+    a.z = __fmul_rn(a.z, f);
+    a.max = max;
+    a.bad = __any_sync(0xffffffffu, a.bad);
 #pragma unroll
     for (int o = 16; o; o /= 2) {
-        Sums b;
-        b.max = __shfl_xor_sync(0xffffffffu, a.max, o);
-        b.z = __shfl_xor_sync(0xffffffffu, a.z, o);
-        b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-        b.bad = __shfl_xor_sync(0xffffffffu, a.bad, o);
-        a = join(a, b, c);
+        a.z = __fadd_rn(a.z, __shfl_xor_sync(0xffffffffu, a.z, o));
+        a.s = __fadd_rn(a.s, __shfl_xor_sync(0xffffffffu, a.s, o));
     }
     return a;
 }
@@ -309,18 +336,35 @@ struct Running {
             ref = fmaxf(ref, m);
         }
     }
-    template <typename T> __device__ __forceinline__ void add(const uint4& raw, float c) {
+    // CLAMP: masked logits may be among them; t is kept at EXP_FLOOR there, where 2^t is 0
+    template <typename T, bool CLAMP> __device__ __forceinline__ void add(const uint4& raw, float c) {
         constexpr int E = 16 / sizeof(T);
         F2 f[E / 2];
         Chunk<T>::get(raw, f);
 #pragma unroll
         for (int e = 0; e < E / 2; ++e) {
             F2 t = mul2(add2(f[e], {-ref, -ref}), {c, c});
-            t = {fmaxf(t.x, EXP_FLOOR), fmaxf(t.y, EXP_FLOOR)};
+            if (CLAMP) t = {fmaxf(t.x, EXP_FLOOR), fmaxf(t.y, EXP_FLOOR)};
             const F2 q = {exp2_fast(t.x), exp2_fast(t.y)};
             z = add2(z, q);
             s = fma2(q, t, s);
         }
+    }
+    // A step's chunks, by all lanes of a warp. The clamp costs a fifth of the arithmetic and only masks need
+    // it: a masked logit makes s NaN (0 * -infinity), and the step is then taken again, and the
+    // warp's later ones, with it.
+    template <typename T, int N> __device__ __forceinline__ void step(const uint4 (&raw)[N], float c, bool& clamp) {
+        if (!clamp) {
+            const F2 z0 = z, s0 = s;
+#pragma unroll
+            for (int u = 0; u < N; ++u) add<T, false>(raw[u], c);
+            const float n = __fadd_rn(s.x, s.y);
+            clamp = __any_sync(0xffffffffu, n != n);
+            if (!clamp) return;
+            z = z0, s = s0;
+        }
+#pragma unroll
+        for (int u = 0; u < N; ++u) add<T, true>(raw[u], c);
     }
     // against the thread's true maximum
     __device__ __forceinline__ Sums sums(float c) const {
@@ -359,114 +403,82 @@ __device__ __forceinline__ void take(unsigned long long& list, unsigned long lon
     bound = k > bound ? k : bound;
 }
 
-// A row to a warp, four to a CTA: rows of up to 512 bytes a lane. The k-th largest of the lanes' maxima is
-// a bound that the k-th best cannot fall below, so few logits are looked at again, from the registers.
-template <typename T> __global__ void __launch_bounds__(128, 8) k_token_logprobs_warp(const LogprobArgs p) {
-    TB_GRID_DEP_ENTRY();
-    constexpr int E = 16 / sizeof(T), U = 4;
-    const int lane = threadIdx.x & 31;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (row >= p.rows) return;
-    const T* x = static_cast<const T*>(p.logits) + row * p.stride;
-    const Row<T> r(x, p.vocab);
-    const int stop = r.chunks();
-    const float c = __fmul_rn(LOG2E, p.inv_t), margin = __fdiv_rn(40.f, c);
-    const float given = given_logit(p, row, x);
-
-    Running a;
-    unsigned long long list = 0, bound = 0;  // bound: keys up to it are not among the `top` best
-    for (int v0 = 0; v0 < stop; v0 += 32 * U) {
-        uint4 raw[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) raw[u] = r.load(v0 + u * 32 + lane, stop);
-        float um[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) um[u] = Chunk<T>::vmax(raw[u]);
-        const float m = max_nan(max_nan(um[0], um[1]), max_nan(um[2], um[3]));
-        a.raise(m, c, margin);
-#pragma unroll
-        for (int u = 0; u < U; ++u) a.add<T>(raw[u], c);
-        if (!p.top) continue;
-        if (v0 == 0) {
-            const uint32_t o = __shfl_sync(0xffffffffu, sort32(ordered(m), lane), p.top - 1);
-            if (unordered(o) > -INFINITY) bound = (unsigned long long)o << 32;
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (!__any_sync(0xffffffffu, um[u] > limit_of(bound))) continue;
-            F2 f[E / 2];
-            Chunk<T>::get(raw[u], f);
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const float v = e & 1 ? f[e / 2].y : f[e / 2].x;
-                const bool in = v > limit_of(bound);
-                if (__any_sync(0xffffffffu, in))
-                    take(list, bound, in ? top_key(v, (uint32_t)((v0 + u * 32 + lane) * E + e - r.head)) : 0ull, p.top, lane);
-            }
-        }
-    }
-    write_row<T>(p, row, join_warp(a.sums(c), c), lane < p.top ? list : 0, given, lane);
-}
-
-// A row, or one of `splits` parts of it, to a CTA. Each step of a thread is a group of U chunks; the groups'
-// maxima stay in shared memory, so that after the one pass only the groups that can hold one of
-// the best are read again: those whose maximum reaches the k-th largest of the threads' maxima, about k of them.
+// NW warps to a row, or to one of `splits` parts of it; a CTA of one warp each: four rows to a CTA. Each step of a
+// thread is a group of U chunks; the groups' maxima stay in shared memory, so that after the one
+// pass only the groups that can hold one of the best are read again: those whose maximum reaches the k-th
+// largest of the threads' maxima, about k of them.
 constexpr int LP_WARPS = 8, LP_U = 4;
 template <typename T> constexpr int LP_STEPS = sizeof(T) == 4 ? 16 : 32;  // most steps of a part
 
-template <typename T> __global__ void __launch_bounds__(LP_WARPS * 32, 4) k_token_logprobs(const LogprobArgs p) {
-    TB_GRID_DEP_ENTRY();
-    constexpr int E = 16 / sizeof(T), U = LP_U, NT = LP_WARPS * 32;
-    __shared__ T group_max[LP_STEPS<T>][NT];
-    __shared__ uint16_t queue[LP_STEPS<T> * NT];
-    __shared__ unsigned long long keys[LP_WARPS][32];
-    __shared__ Sums wsums[LP_WARPS];
-    __shared__ unsigned long long shared_bound;
-    __shared__ int queued, last;
+template <typename T, int NW> struct RowShared {
+    T group_max[LP_STEPS<T>][NW * 32];
+    uint16_t queue[LP_STEPS<T> * NW * 32];
+    unsigned long long keys[NW][32];
+    Sums sums[NW];
+    unsigned long long bound;
+    int queued, last;
+};
 
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t row = (int64_t)blockIdx.x / p.splits;
-    const int split = (int)((int64_t)blockIdx.x - row * p.splits);
+template <int NW> __device__ __forceinline__ void row_sync() {
+    if constexpr (NW == 1) __syncwarp();
+    else __syncthreads();
+}
+
+template <typename T, int NW> __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 8 : 4) k_token_logprobs(const LogprobArgs p) {
+    TB_GRID_DEP_ENTRY();
+    constexpr int E = 16 / sizeof(T), U = LP_U, NT = NW * 32, ROWS = NW == 1 ? 4 : 1;
+    __shared__ RowShared<T, NW> shared[ROWS];
+    RowShared<T, NW>& sh = shared[NW == 1 ? threadIdx.x >> 5 : 0];
+
+    const int lane = threadIdx.x & 31, warp = NW == 1 ? 0 : threadIdx.x >> 5, tid = warp * 32 + lane;
+    const int64_t unit = NW == 1 ? (int64_t)blockIdx.x * ROWS + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
+    const int64_t row = NW == 1 ? unit : unit / p.splits;
+    if (NW == 1 && row >= p.rows) return;
+    const int split = NW == 1 ? 0 : (int)(unit - row * p.splits);
     const T* x = static_cast<const T*>(p.logits) + row * p.stride;
     const Row<T> r(x, p.vocab);
-    const int chunks = r.chunks(), per = (int)(((int64_t)chunks + p.splits - 1) / p.splits);
+    const int chunks = r.chunks(), per = NW == 1 ? chunks : (int)(((int64_t)chunks + p.splits - 1) / p.splits);
     const int begin = (int)min((int64_t)chunks, (int64_t)split * per), stop = min(chunks, begin + per);
     const float c = __fmul_rn(LOG2E, p.inv_t), margin = __fdiv_rn(40.f, c);
+
     const float given = warp == 0 ? given_logit(p, row, x) : 0.f;
-    if (tid == 0) queued = 0;
+    if (tid == 0) sh.queued = 0;
 
     Running a;
     int steps = 0;
+    bool clamp = false;
     for (int v0 = begin; v0 < stop; v0 += NT * U, ++steps) {
         uint4 raw[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) raw[u] = r.load(v0 + u * NT + tid, stop);
-        float m = Chunk<T>::vmax(raw[0]);
-#pragma unroll
-        for (int u = 1; u < U; ++u) m = max_nan(m, Chunk<T>::vmax(raw[u]));
-        if (p.top) group_max[steps][tid] = Elem<T>::put(m);  // exact: m is one of the logits
+        r.step(raw, v0, tid, NT, stop);
+        const float m = Chunk<T>::vmax(raw);
+        if (p.top) sh.group_max[steps][tid] = Elem<T>::put(m);  // exact: m is one of the logits
         a.raise(m, c, margin);
-#pragma unroll
-        for (int u = 0; u < U; ++u) a.add<T>(raw[u], c);
+        a.template step<T>(raw, c, clamp);
     }
     Sums w = join_warp(a.sums(c), c);
-    if (lane == 0) wsums[warp] = w;
     unsigned long long list = 0;
+    if (NW > 1 && lane == 0) sh.sums[warp] = w;
     if (p.top) {
-        uint32_t o = merge_warps<LP_WARPS>(sort32(ordered(a.max), lane), reinterpret_cast<uint32_t (*)[32]>(keys), warp, lane);
-        if (warp == 0) {
+        uint32_t o = sort32(ordered(a.max), lane);
+        if constexpr (NW > 1) {
+            o = merge_warps<NW>(o, reinterpret_cast<uint32_t (*)[32]>(sh.keys), warp, lane);
+            if (warp == 0) {
+                o = __shfl_sync(0xffffffffu, o, p.top - 1);
+                if (lane == 0) sh.bound = unordered(o) > -INFINITY ? (unsigned long long)o << 32 : 0;
+            }
+        } else {
             o = __shfl_sync(0xffffffffu, o, p.top - 1);
-            if (lane == 0) shared_bound = unordered(o) > -INFINITY ? (unsigned long long)o << 32 : 0;
+            if (lane == 0) sh.bound = unordered(o) > -INFINITY ? (unsigned long long)o << 32 : 0;
         }
-        __syncthreads();
-        unsigned long long bound = shared_bound;
+        row_sync<NW>();
+        unsigned long long bound = sh.bound;
         const float limit = limit_of(bound);
         for (int i = 0; i < steps; ++i)
-            if (Elem<T>::get(group_max[i][tid]) > limit) queue[atomicAdd(&queued, 1)] = (uint16_t)(i * NT + tid);
-        __syncthreads();
-        const int n = queued;
-        for (int q = warp; q < n; q += LP_WARPS) {
-            const int g = queue[q];
+            if (Elem<T>::get(sh.group_max[i][tid]) > limit) sh.queue[atomicAdd(&sh.queued, 1)] = (uint16_t)(i * NT + tid);
+        row_sync<NW>();
+        const int n = sh.queued;
+        for (int q = warp; q < n; q += NW) {
+            const int g = sh.queue[q];
             // an element a lane; every lane takes part in take(), also those past the group's U * E
             static_assert(U * E <= 32, "a group is read by one warp at a time");
             const int v = begin + (g / NT) * NT * U + (lane / E) * NT + g % NT;
@@ -475,36 +487,39 @@ template <typename T> __global__ void __launch_bounds__(LP_WARPS * 32, 4) k_toke
             const float l = in ? Elem<T>::get(r.base[at]) : -INFINITY;
             take(list, bound, l > limit ? top_key(l, (uint32_t)(at - r.head)) : 0ull, p.top, lane);
         }
-        list = merge_warps<LP_WARPS>(lane < p.top ? list : 0ull, keys, warp, lane);
+        if (lane >= p.top) list = 0;
+        if constexpr (NW > 1) list = merge_warps<NW>(list, sh.keys, warp, lane);
     } else {
-        __syncthreads();
+        row_sync<NW>();
     }
-    if (warp == 0) w = join_warp(lane < LP_WARPS ? wsums[lane] : Sums{-INFINITY, 0.f, 0.f, 0}, c);
-    if (p.splits > 1) {
-        Part* part = p.parts + row * p.splits;
-        if (warp == 0) {
-            if (lane == 0) part[split].sums = w;
-            part[split].keys[lane] = list;
-            __threadfence();
-            __syncwarp();
-            if (lane == 0) {
-                last = atomicAdd(&p.counters[row], 1) == p.splits - 1;
-                if (last) p.counters[row] = 0;  // ready for the next launch
+    if constexpr (NW > 1) {
+        if (warp == 0) w = join_warp(lane < NW ? sh.sums[lane] : Sums{-INFINITY, 0.f, 0.f, 0}, c);
+        if (p.splits > 1) {
+            Part* part = p.parts + row * p.splits;
+            if (warp == 0) {
+                if (lane == 0) part[split].sums = w;
+                part[split].keys[lane] = list;
+                __threadfence();
+                __syncwarp();
+                if (lane == 0) {
+                    sh.last = atomicAdd(&p.counters[row], 1) == p.splits - 1;
+                    if (sh.last) p.counters[row] = 0;  // ready for the next launch
+                }
             }
+            __syncthreads();
+            if (!sh.last) return;
+            __threadfence();
+            w = {-INFINITY, 0.f, 0.f, 0};
+            list = 0;
+            for (int i = warp; i < p.splits; i += NW) {
+                w = join(w, {__ldcg(&part[i].sums.max), __ldcg(&part[i].sums.z), __ldcg(&part[i].sums.s), __ldcg(&part[i].sums.bad)}, c);
+                if (p.top) list = merge32(list, __ldcg(&part[i].keys[lane]), lane);
+            }
+            if (lane == 0) sh.sums[warp] = w;
+            __syncthreads();
+            if (p.top) list = merge_warps<NW>(list, sh.keys, warp, lane);
+            if (warp == 0) w = join_warp(lane < NW ? sh.sums[lane] : Sums{-INFINITY, 0.f, 0.f, 0}, c);
         }
-        __syncthreads();
-        if (!last) return;
-        __threadfence();
-        w = {-INFINITY, 0.f, 0.f, 0};
-        list = 0;
-        for (int i = warp; i < p.splits; i += LP_WARPS) {
-            w = join(w, {__ldcg(&part[i].sums.max), __ldcg(&part[i].sums.z), __ldcg(&part[i].sums.s), __ldcg(&part[i].sums.bad)}, c);
-            if (p.top) list = merge32(list, __ldcg(&part[i].keys[lane]), lane);
-        }
-        if (lane == 0) wsums[warp] = w;
-        __syncthreads();
-        if (p.top) list = merge_warps<LP_WARPS>(list, keys, warp, lane);
-        if (warp == 0) w = join_warp(lane < LP_WARPS ? wsums[lane] : Sums{-INFINITY, 0.f, 0.f, 0}, c);
     }
     if (warp == 0) write_row<T>(p, row, w, list, given, lane);
 }
@@ -512,16 +527,17 @@ template <typename T> __global__ void __launch_bounds__(LP_WARPS * 32, 4) k_toke
 template <typename T> int launch_logprobs(tb_ctx* ctx, LogprobArgs p) {
     constexpr int E = 16 / sizeof(T);
     const int64_t chunks = ceil_div(p.vocab, E) + 1;  // one more where a row starts inside a chunk
-    // a warp per row while a row is at most a step of it: @@W@@
-    if (chunks <= 32 * 4 + 1)
-        return launch(ctx, "k_token_logprobs_warp", k_token_logprobs_warp<T>, dim3((unsigned)ceil_div(p.rows, 4)), dim3(128), 0, p);
+    const int64_t step = 32 * LP_U;                   // chunks a step of one warp
+    // a warp per row while a row is one step of it, or the rows are enough to fill the GPU with warps: @@W@@
+    if (chunks <= step + 1 || (p.rows >= 16 * ctx->sm_count && chunks <= step * 16))
+        return launch(ctx, "k_token_logprobs", k_token_logprobs<T, 1>, dim3((unsigned)ceil_div(p.rows, 4)), dim3(128), 0, p);
     // a row in parts of a step each at least while the CTAs do not fill the GPU four times over, and of LP_STEPS at
     // most
-    const int64_t step = LP_WARPS * 32 * LP_U, steps = ceil_div(chunks, step);
+    const int64_t steps = ceil_div(chunks, step * LP_WARPS);
     p.splits = (int)std::max<int64_t>(std::min<int64_t>({steps, 4 * ctx->sm_count / p.rows, 256}), ceil_div(steps, LP_STEPS<T>));
     if (p.rows * p.splits > 2147483647) return fail(TB_ERR_UNSUPPORTED, "token logprobs: too many rows");
     if (p.splits > 1) {
-        // partial results and counters (zeroed: the context's own are too few for many long rows)
+        // partial results and counters (the context's own, always left at 0, are too few for many long rows)
         const size_t parts = (size_t)(p.rows * p.splits) * sizeof(Part);
         const bool own = p.rows > ctx->tile_cnt_len;
         const int r = ensure_workspace(ctx, parts + (own ? p.rows * sizeof(int) : 0));
@@ -533,7 +549,7 @@ template <typename T> int launch_logprobs(tb_ctx* ctx, LogprobArgs p) {
             TB_CHECK_CUDA(cudaMemsetAsync(p.counters, 0, p.rows * sizeof(int), ctx->stream));
         }
     }
-    return launch(ctx, "k_token_logprobs", k_token_logprobs<T>, dim3((unsigned)(p.rows * p.splits)), dim3(LP_WARPS * 32), 0, p);
+    return launch(ctx, "k_token_logprobs", k_token_logprobs<T, LP_WARPS>, dim3((unsigned)(p.rows * p.splits)), dim3(LP_WARPS * 32), 0, p);
 }
 
 // ---- gradient ---------------------------------------------------------------------------------------
