@@ -185,17 +185,27 @@ template <typename T> struct Row {
         }
         return r;
     }
-    // chunks v0 + u * apart + at, u < N, of a step that begins at chunk v0 (the same for all its threads) and
-    // spans N * apart of them: most steps are whole and need no check for a chunk
-    template <int N> __device__ __forceinline__ void step(uint4 (&r)[N], int v0, int at, int apart, int stop) const {
-        if (whole(v0) && v0 + N * apart <= min(stop, end / E)) {
-            const uint4* q = reinterpret_cast<const uint4*>(base) + v0 + at;
+    // Chunks v0 + u * apart + at, u < N, of a step that begins at chunk v0 (the same for all its threads) and
+    // spans N * apart of them; false for a step at the row's edge, where some are masked.
+    template <int N> __device__ __forceinline__ bool step(uint4 (&r)[N], int v0, int at, int apart, int stop) const {
+        const int whole_end = min(stop, end / E), next = v0 + N * apart;
+        const uint4* q = reinterpret_cast<const uint4*>(base) + v0 + at;
+        if ((v0 > 0 || head == 0) && next <= whole_end) {
 #pragma unroll
             for (int u = 0; u < N; ++u) r[u] = q[u * apart];
+            return true;
+        }
+        if ((v0 > 0 || head == 0) && whole_end == stop) {  // every chunk whole or outside
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                r[u] = make_uint4(Chunk<T>::MASKED, Chunk<T>::MASKED, Chunk<T>::MASKED, Chunk<T>::MASKED);
+                if (v0 + u * apart + at < stop) r[u] = q[u * apart];
+            }
         } else {
 #pragma unroll
             for (int u = 0; u < N; ++u) r[u] = load(v0 + u * apart + at, stop);
         }
+        return false;
     }
 };
 
@@ -278,19 +288,27 @@ struct Part {
     unsigned long long keys[TOP_MAX];
 };
 
+// A row's given token and its logit, read before the pass so that the row's end does not wait for them.
+struct Given {
+    int64_t token = -1;
+    float logit = 0.f;
+    template <typename T> __device__ __forceinline__ void read(const LogprobArgs& p, int64_t row, const T* x) {
+        if (!p.logprob) return;
+        token = p.tokens[row];
+        if (token >= 0 && token < p.vocab) logit = Elem<T>::get(x[token]);
+    }
+};
+
 // Results of one row, by one warp that holds its sums and its best keys.
-template <typename T>
-__device__ __forceinline__ void write_row(const LogprobArgs& p, int64_t row, const Sums& a, unsigned long long list, float given, int lane) {
+__device__ __forceinline__ void write_row(const LogprobArgs& p, int64_t row, const Sums& a, unsigned long long list, const Given& given, int lane) {
     const bool empty = a.max == -INFINITY;
     const float logz = logf(a.z);
     auto logprob = [&](float v) {
         return a.bad ? nan_f() : empty ? -INFINITY : __fsub_rn(__fmul_rn(__fsub_rn(v, a.max), p.inv_t), logz);
     };
     if (lane == 0) {
-        if (p.logprob) {
-            const int64_t t = p.tokens[row];
-            p.logprob[row] = t >= p.vocab ? nan_f() : t < 0 ? (a.bad ? nan_f() : 0.f) : logprob(given);
-        }
+        if (p.logprob)
+            p.logprob[row] = given.token >= p.vocab ? nan_f() : given.token < 0 ? (a.bad ? nan_f() : 0.f) : logprob(given.logit);
         if (p.entropy)
             p.entropy[row] = a.bad ? nan_f() : empty ? 0.f : fmaxf(__fsub_rn(logz, __fmul_rn(__fdiv_rn(a.s, a.z), LN2)), 0.f);
         if (p.lse) p.lse[row] = a.bad ? nan_f() : empty ? -INFINITY : __fadd_rn(__fmul_rn(a.max, p.inv_t), logz);
@@ -350,21 +368,22 @@ struct Running {
             s = fma2(q, t, s);
         }
     }
-    // A step's chunks, by all lanes of a warp. The clamp costs a fifth of the arithmetic and only masks need
-    // it: a masked logit makes s NaN (0 * -infinity), and the step is then taken again, and the
-    // warp's later ones, with it.
-    template <typename T, int N> __device__ __forceinline__ void step(const uint4 (&raw)[N], float c, bool& clamp) {
-        if (!clamp) {
+    // A step's chunks, by all lanes of a warp; the first `n` of them are not empty for all. The clamp costs a fifth
+    // of the arithmetic and only masks need it: the row's edge has some, and elsewhere a masked logit
+    // makes s NaN (0 * -infinity), and the step is then taken again, and the warp's later ones, with it.
+    template <typename T, int N> __device__ __forceinline__ void step(const uint4 (&raw)[N], int n, float c, bool edge, bool& clamp) {
+        if (!clamp && !edge) {
             const F2 z0 = z, s0 = s;
 #pragma unroll
             for (int u = 0; u < N; ++u) add<T, false>(raw[u], c);
-            const float n = __fadd_rn(s.x, s.y);
-            clamp = __any_sync(0xffffffffu, n != n);
+            const float t = __fadd_rn(s.x, s.y);
+            clamp = __any_sync(0xffffffffu, t != t);
             if (!clamp) return;
             z = z0, s = s0;
         }
 #pragma unroll
-        for (int u = 0; u < N; ++u) add<T, true>(raw[u], c);
+        for (int u = 0; u < N; ++u)
+            if (u < n) add<T, true>(raw[u], c);
     }
     // against the thread's true maximum
     __device__ __forceinline__ Sums sums(float c) const {
@@ -373,12 +392,6 @@ struct Running {
         return {max, __fmul_rn(zz, f), __fmul_rn(fmaf(zz, d, ss), f), bad};
     }
 };
-
-template <typename T> __device__ __forceinline__ float given_logit(const LogprobArgs& p, int64_t row, const T* x) {
-    if (!p.logprob) return 0.f;
-    const int64_t t = p.tokens[row];
-    return t >= 0 && t < p.vocab ? Elem<T>::get(x[t]) : 0.f;
-}
 
 // The largest float below the value of a bound's key, so that `logit > limit_of(bound)` lets in equal logits
 // at lower columns; -infinity for no bound.
@@ -407,7 +420,7 @@ __device__ __forceinline__ void take(unsigned long long& list, unsigned long lon
 // thread is a group of U chunks; the groups' maxima stay in shared memory, so that after the one
 // pass only the groups that can hold one of the best are read again: those whose maximum reaches the k-th
 // largest of the threads' maxima, about k of them.
-constexpr int LP_WARPS = 8, LP_U = 4;
+constexpr int LP_U = 4;
 template <typename T> constexpr int LP_STEPS = sizeof(T) == 4 ? 16 : 32;  // most steps of a part
 
 template <typename T, int NW> struct RowShared {
@@ -424,7 +437,7 @@ template <int NW> __device__ __forceinline__ void row_sync() {
     else __syncthreads();
 }
 
-template <typename T, int NW> __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 8 : 4) k_token_logprobs(const LogprobArgs p) {
+template <typename T, int NW> __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 8 : 32 / NW) k_token_logprobs(const LogprobArgs p) {
     TB_GRID_DEP_ENTRY();
     constexpr int E = 16 / sizeof(T), U = LP_U, NT = NW * 32, ROWS = NW == 1 ? 4 : 1;
     __shared__ RowShared<T, NW> shared[ROWS];
@@ -441,7 +454,8 @@ template <typename T, int NW> __global__ void __launch_bounds__(NW == 1 ? 128 : 
     const int begin = (int)min((int64_t)chunks, (int64_t)split * per), stop = min(chunks, begin + per);
     const float c = __fmul_rn(LOG2E, p.inv_t), margin = __fdiv_rn(40.f, c);
 
-    const float given = warp == 0 ? given_logit(p, row, x) : 0.f;
+    Given given;
+    if (warp == 0) given.read(p, row, x);
     if (tid == 0) sh.queued = 0;
 
     Running a;
@@ -449,11 +463,11 @@ template <typename T, int NW> __global__ void __launch_bounds__(NW == 1 ? 128 : 
     bool clamp = false;
     for (int v0 = begin; v0 < stop; v0 += NT * U, ++steps) {
         uint4 raw[U];
-        r.step(raw, v0, tid, NT, stop);
+        const bool whole = r.step(raw, v0, tid, NT, stop);
         const float m = Chunk<T>::vmax(raw);
         if (p.top) sh.group_max[steps][tid] = Elem<T>::put(m);  // exact: m is one of the logits
         a.raise(m, c, margin);
-        a.template step<T>(raw, c, clamp);
+        a.template step<T>(raw, (stop - v0 + NT - 1) / NT, c, !whole, clamp);
     }
     Sums w = join_warp(a.sums(c), c);
     unsigned long long list = 0;
@@ -477,15 +491,22 @@ template <typename T, int NW> __global__ void __launch_bounds__(NW == 1 ? 128 : 
             if (Elem<T>::get(sh.group_max[i][tid]) > limit) sh.queue[atomicAdd(&sh.queued, 1)] = (uint16_t)(i * NT + tid);
         row_sync<NW>();
         const int n = sh.queued;
-        for (int q = warp; q < n; q += NW) {
-            const int g = sh.queue[q];
-            // an element a lane; every lane takes part in take(), also those past the group's U * E
-            static_assert(U * E <= 32, "a group is read by one warp at a time");
-            const int v = begin + (g / NT) * NT * U + (lane / E) * NT + g % NT;
-            const int64_t at = (int64_t)v * E + lane % E;
-            const bool in = lane < U * E && v < stop && at >= r.head && at < r.end;
-            const float l = in ? Elem<T>::get(r.base[at]) : -INFINITY;
-            take(list, bound, l > limit ? top_key(l, (uint32_t)(at - r.head)) : 0ull, p.top, lane);
+        // an element a lane; every lane takes part in take(), also those past a group's U * E
+        static_assert(U * E <= 32, "a group is read by one warp at a time");
+        for (int q = warp; q < n; q += 4 * NW) {
+            float l[4];
+            int at[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {  // the loads of four groups at once
+                const int g = sh.queue[min(q + j * NW, n - 1)];
+                const int v = begin + (g / NT) * NT * U + (lane / E) * NT + g % NT;
+                at[j] = v * E + lane % E;
+                const bool in = q + j * NW < n && lane < U * E && v < stop && at[j] >= r.head && at[j] < r.end;
+                l[j] = in ? Elem<T>::get(r.base[at[j]]) : -INFINITY;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (q + j * NW < n) take(list, bound, l[j] > limit ? top_key(l[j], (uint32_t)(at[j] - r.head)) : 0ull, p.top, lane);
         }
         if (lane >= p.top) list = 0;
         if constexpr (NW > 1) list = merge_warps<NW>(list, sh.keys, warp, lane);
@@ -521,20 +542,21 @@ template <typename T, int NW> __global__ void __launch_bounds__(NW == 1 ? 128 : 
             if (warp == 0) w = join_warp(lane < NW ? sh.sums[lane] : Sums{-INFINITY, 0.f, 0.f, 0}, c);
         }
     }
-    if (warp == 0) write_row<T>(p, row, w, list, given, lane);
+    if (warp == 0) write_row(p, row, w, list, given, lane);
 }
 
 template <typename T> int launch_logprobs(tb_ctx* ctx, LogprobArgs p) {
     constexpr int E = 16 / sizeof(T);
     const int64_t chunks = ceil_div(p.vocab, E) + 1;  // one more where a row starts inside a chunk
     const int64_t step = 32 * LP_U;                   // chunks a step of one warp
-    // a warp per row while a row is one step of it, or the rows are enough to fill the GPU with warps: @@W@@
-    if (chunks <= step + 1 || (p.rows >= 16 * ctx->sm_count && chunks <= step * 16))
-        return launch(ctx, "k_token_logprobs", k_token_logprobs<T, 1>, dim3((unsigned)ceil_div(p.rows, 4)), dim3(128), 0, p);
-    // a row in parts of a step each at least while the CTAs do not fill the GPU four times over, and of LP_STEPS at
-    // most
-    const int64_t steps = ceil_div(chunks, step * LP_WARPS);
-    p.splits = (int)std::max<int64_t>(std::min<int64_t>({steps, 4 * ctx->sm_count / p.rows, 256}), ceil_div(steps, LP_STEPS<T>));
+    // Warps per row: the fewest (they share the work at a row's end, which the others wait for) that keep
+    // 20 warps on every SM and a part within LP_STEPS steps: @@W@@
+    int nw = 1;
+    while (nw < 8 && chunks > step * nw + 1 && (p.rows * nw < 20 * ctx->sm_count || chunks > step * nw * LP_STEPS<T>)) nw *= 2;
+    // with 8 a row goes in parts of a step each at least while the CTAs do not fill the GPU, and of LP_STEPS at most
+    const int64_t steps = ceil_div(chunks, step * nw);
+    p.splits = 1;
+    if (nw == 8) p.splits = (int)std::max<int64_t>(std::min<int64_t>({steps, 4 * ctx->sm_count / p.rows, 256}), ceil_div(steps, LP_STEPS<T>));
     if (p.rows * p.splits > 2147483647) return fail(TB_ERR_UNSUPPORTED, "token logprobs: too many rows");
     if (p.splits > 1) {
         // partial results and counters (the context's own, always left at 0, are too few for many long rows)
@@ -549,7 +571,13 @@ template <typename T> int launch_logprobs(tb_ctx* ctx, LogprobArgs p) {
             TB_CHECK_CUDA(cudaMemsetAsync(p.counters, 0, p.rows * sizeof(int), ctx->stream));
         }
     }
-    return launch(ctx, "k_token_logprobs", k_token_logprobs<T, LP_WARPS>, dim3((unsigned)(p.rows * p.splits)), dim3(LP_WARPS * 32), 0, p);
+    const dim3 grid((unsigned)(nw == 1 ? ceil_div(p.rows, 4) : p.rows * p.splits)), block((unsigned)(nw == 1 ? 128 : nw * 32));
+    switch (nw) {
+    case 1: return launch(ctx, "k_token_logprobs", k_token_logprobs<T, 1>, grid, block, 0, p);
+    case 2: return launch(ctx, "k_token_logprobs", k_token_logprobs<T, 2>, grid, block, 0, p);
+    case 4: return launch(ctx, "k_token_logprobs", k_token_logprobs<T, 4>, grid, block, 0, p);
+    default: return launch(ctx, "k_token_logprobs", k_token_logprobs<T, 8>, grid, block, 0, p);
+    }
 }
 
 // ---- gradient ---------------------------------------------------------------------------------------
