@@ -106,6 +106,11 @@ template <> struct Chunk<float> {
             m = max_nan(m, max_nan(max_nan(__uint_as_float(r[i].x), __uint_as_float(r[i].y)), max_nan(__uint_as_float(r[i].z), __uint_as_float(r[i].w))));
         return m;
     }
+    // bit e: logit e is at least v
+    static __device__ __forceinline__ uint32_t at_least(const uint4& r, float v) {
+        return (__uint_as_float(r.x) >= v ? 1u : 0u) | (__uint_as_float(r.y) >= v ? 2u : 0u) | (__uint_as_float(r.z) >= v ? 4u : 0u) |
+               (__uint_as_float(r.w) >= v ? 8u : 0u);
+    }
     static __device__ __forceinline__ void get(const uint4& r, F2* f) {
         f[0] = {__uint_as_float(r.x), __uint_as_float(r.y)};
         f[1] = {__uint_as_float(r.z), __uint_as_float(r.w)};
@@ -125,6 +130,12 @@ template <> struct Chunk<__nv_bfloat16> {
         for (int i = 1; i < N; ++i) m[0] = __hmax2_nan(m[0], m[i]);
         return max_nan(__low2float(m[0]), __high2float(m[0]));
     }
+    static __device__ __forceinline__ uint32_t at_least(const uint4& r, float v) {
+        const __nv_bfloat162 l = __float2bfloat162_rn(v);  // exact: v is a logit of this type
+        auto ge = [&](uint32_t w) { return __hge2_mask(*reinterpret_cast<const __nv_bfloat162*>(&w), l); };
+        const uint32_t m = (ge(r.x) & 0x00020001u) | (ge(r.y) & 0x00080004u) | (ge(r.z) & 0x00200010u) | (ge(r.w) & 0x00800040u);
+        return (m | m >> 16) & 0xffu;
+    }
     static __device__ __forceinline__ F2 two(uint32_t w) { return {__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)}; }
     static __device__ __forceinline__ void get(const uint4& r, F2* f) { f[0] = two(r.x), f[1] = two(r.y), f[2] = two(r.z), f[3] = two(r.w); }
     static __device__ __forceinline__ uint32_t one(F2 a) {
@@ -143,6 +154,12 @@ template <> struct Chunk<__half> {
 #pragma unroll
         for (int i = 1; i < N; ++i) m[0] = __hmax2_nan(m[0], m[i]);
         return max_nan(__low2float(m[0]), __high2float(m[0]));
+    }
+    static __device__ __forceinline__ uint32_t at_least(const uint4& r, float v) {
+        const __half2 l = __float2half2_rn(v);  // exact: v is a logit of this type
+        auto ge = [&](uint32_t w) { return __hge2_mask(*reinterpret_cast<const __half2*>(&w), l); };
+        const uint32_t m = (ge(r.x) & 0x00020001u) | (ge(r.y) & 0x00080004u) | (ge(r.z) & 0x00200010u) | (ge(r.w) & 0x00800040u);
+        return (m | m >> 16) & 0xffu;
     }
     static __device__ __forceinline__ F2 two(uint32_t w) {
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
@@ -222,6 +239,16 @@ template <typename K> __device__ __forceinline__ K sort32(K a, int lane) {
             a = up == (a > b) ? a : b;
         }
     return a;
+}
+// The k-th largest of 32 values, or a smaller one where some are equal: a bound that at least k reach.
+__device__ __forceinline__ uint32_t kth32(uint32_t a, int k, int lane) {
+    if (k > 8) return __shfl_sync(0xffffffffu, sort32(a, lane), k - 1);
+    uint32_t m = 0;
+    for (int i = 0; i < k; ++i) {
+        m = __reduce_max_sync(0xffffffffu, a);
+        if (a == m) a = 0;
+    }
+    return m;
 }
 // the 32 largest of two descending lists, descending
 template <typename K> __device__ __forceinline__ K merge32(K a, K b, int lane) {
@@ -423,13 +450,16 @@ __device__ __forceinline__ void take(unsigned long long& list, unsigned long lon
 constexpr int LP_U = 4;
 template <typename T> constexpr int LP_STEPS = sizeof(T) == 4 ? 16 : 32;  // most steps of a part
 
+constexpr int KEYS = 64;  // candidates that are ranked against one another
+
 template <typename T, int NW> struct RowShared {
     T group_max[LP_STEPS<T>][NW * 32];
     uint16_t queue[LP_STEPS<T> * NW * 32];
     unsigned long long keys[NW][32];
     Sums sums[NW];
+    unsigned long long found[KEYS], ranked[32];
     unsigned long long bound;
-    int queued, last;
+    int queued, nfound, last;
 };
 
 template <int NW> __device__ __forceinline__ void row_sync() {
@@ -456,13 +486,13 @@ template <typename T, int NW> __global__ void __launch_bounds__(NW == 1 ? 128 : 
 
     Given given;
     if (warp == 0) given.read(p, row, x);
-    if (tid == 0) sh.queued = 0;
+    if (tid == 0) sh.queued = sh.nfound = 0;
 
     Running a;
     int steps = 0;
     bool clamp = false;
+    uint4 raw[U];
     for (int v0 = begin; v0 < stop; v0 += NT * U, ++steps) {
-        uint4 raw[U];
         const bool whole = r.step(raw, v0, tid, NT, stop);
         const float m = Chunk<T>::vmax(raw);
         if (p.top) sh.group_max[steps][tid] = Elem<T>::put(m);  // exact: m is one of the logits
@@ -473,43 +503,95 @@ template <typename T, int NW> __global__ void __launch_bounds__(NW == 1 ? 128 : 
     unsigned long long list = 0;
     if (NW > 1 && lane == 0) sh.sums[warp] = w;
     if (p.top) {
-        uint32_t o = sort32(ordered(a.max), lane);
+        uint32_t o = ordered(a.max);
         if constexpr (NW > 1) {
+            o = sort32(o, lane);
             o = merge_warps<NW>(o, reinterpret_cast<uint32_t (*)[32]>(sh.keys), warp, lane);
             if (warp == 0) {
                 o = __shfl_sync(0xffffffffu, o, p.top - 1);
                 if (lane == 0) sh.bound = unordered(o) > -INFINITY ? (unsigned long long)o << 32 : 0;
             }
         } else {
-            o = __shfl_sync(0xffffffffu, o, p.top - 1);
+            o = kth32(o, p.top, lane);
             if (lane == 0) sh.bound = unordered(o) > -INFINITY ? (unsigned long long)o << 32 : 0;
         }
         row_sync<NW>();
         unsigned long long bound = sh.bound;
         const float limit = limit_of(bound);
-        for (int i = 0; i < steps; ++i)
-            if (Elem<T>::get(sh.group_max[i][tid]) > limit) sh.queue[atomicAdd(&sh.queued, 1)] = (uint16_t)(i * NT + tid);
-        row_sync<NW>();
-        const int n = sh.queued;
-        // an element a lane; every lane takes part in take(), also those past a group's U * E
+        auto queue_groups = [&] {
+            for (int i = 0; i < steps; ++i)
+                if (Elem<T>::get(sh.group_max[i][tid]) > limit) sh.queue[atomicAdd(&sh.queued, 1)] = (uint16_t)(i * NT + tid);
+            row_sync<NW>();
+            return sh.queued;
+        };
+        // the groups q, q + NW, .. < q + 4 NW of the queue, an element a lane, four loads at once; every lane takes part
+        // in f, also those past a group's U * E
         static_assert(U * E <= 32, "a group is read by one warp at a time");
-        for (int q = warp; q < n; q += 4 * NW) {
-            float l[4];
-            int at[4];
+        auto read_groups = [&](int n, auto f) {
+            for (int q = warp; q < n; q += 4 * NW) {
+                float l[4];
+                int at[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {  // the loads of four groups at once
-                const int g = sh.queue[min(q + j * NW, n - 1)];
-                const int v = begin + (g / NT) * NT * U + (lane / E) * NT + g % NT;
-                at[j] = v * E + lane % E;
-                const bool in = q + j * NW < n && lane < U * E && v < stop && at[j] >= r.head && at[j] < r.end;
-                l[j] = in ? Elem<T>::get(r.base[at[j]]) : -INFINITY;
+                for (int j = 0; j < 4; ++j) {
+                    const int g = sh.queue[min(q + j * NW, n - 1)];
+                    const int v = begin + (g / NT) * NT * U + (lane / E) * NT + g % NT;
+                    at[j] = v * E + lane % E;
+                    const bool in = q + j * NW < n && lane < U * E && v < stop && at[j] >= r.head && at[j] < r.end;
+                    l[j] = in ? Elem<T>::get(r.base[at[j]]) : -INFINITY;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (q + j * NW < n) f(l[j] > limit ? top_key(l[j], (uint32_t)(at[j] - r.head)) : 0ull);
             }
+        };
+        auto found = [&](unsigned long long key) {
+            const int i = atomicAdd(&sh.nfound, 1);
+            if (i < KEYS) sh.found[i] = key;
+        };
+        int groups = -1;
+        if (steps == 1 && bound) {  // the logits are still in registers
+            const float v = key_val(bound);
+            if (a.max >= v) {
+                uint32_t some = 0;  // bit u * E + e
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (q + j * NW < n) take(list, bound, l[j] > limit ? top_key(l[j], (uint32_t)(at[j] - r.head)) : 0ull, p.top, lane);
+                for (int u = 0; u < U; ++u) some |= Chunk<T>::at_least(raw[u], v) << u * E;
+                while (some) {
+                    const int i = __ffs((int)some) - 1;
+                    some &= some - 1;
+                    const int at = (begin + (i / E) * NT + tid) * E + i % E;
+                    found(top_key(Elem<T>::get(r.base[at]), (uint32_t)(at - r.head)));
+                }
+            }
+        } else {
+            groups = queue_groups();
+            read_groups(groups, [&](unsigned long long key) {
+                if (key) found(key);
+            });
         }
-        if (lane >= p.top) list = 0;
-        if constexpr (NW > 1) list = merge_warps<NW>(list, sh.keys, warp, lane);
+        row_sync<NW>();
+        const int n = sh.nfound;
+        if (n <= KEYS) {
+            // few: each is placed by the number of larger ones
+            if (warp == 0) {
+                const unsigned long long k0 = lane < n ? sh.found[lane] : 0, k1 = lane + 32 < n ? sh.found[lane + 32] : 0;
+                int r0 = 0, r1 = 0;
+                for (int i = 0; i < n; ++i) {
+                    const unsigned long long k = sh.found[i];
+                    r0 += k > k0;
+                    r1 += k > k1;
+                }
+                if (lane < n && r0 < 32) sh.ranked[r0] = k0;
+                if (lane + 32 < n && r1 < 32) sh.ranked[r1] = k1;
+                __syncwarp();
+                list = lane < min(n, p.top) ? sh.ranked[lane] : 0;
+            }
+        } else {
+            // many equal logits, or few distinct ones: through the warps' sorted lists
+            if (groups < 0) groups = queue_groups();
+            read_groups(groups, [&](unsigned long long key) { take(list, bound, key, p.top, lane); });
+            if (lane >= p.top) list = 0;
+            if constexpr (NW > 1) list = merge_warps<NW>(list, sh.keys, warp, lane);
+        }
     } else {
         row_sync<NW>();
     }
