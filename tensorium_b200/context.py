@@ -25,6 +25,7 @@ class Context:
         check(lib.tb_init(self.device, C.byref(opts), C.byref(self.handle)))
         self.torch_device = torch.device("cuda", self.device)
         self.stream = None
+        self._raw = lib.tb_get_stream(self.handle) or 0
         self._dependents = weakref.WeakSet()  # objects holding library handles tied to this context
         if use_torch_stream:
             self.set_stream(torch.cuda.current_stream(self.device))
@@ -34,11 +35,12 @@ class Context:
         raw = stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
         check(lib.tb_set_stream(self.handle, C.c_void_p(raw)))
         self.stream = stream
+        self._raw = raw
 
     @property
     def raw_stream(self) -> int:
         """cudaStream_t that the context launches on (0: the legacy default stream)."""
-        return lib.tb_get_stream(self.handle) or 0
+        return self._raw
 
     def sync(self) -> None:
         check(lib.tb_sync(self.handle))

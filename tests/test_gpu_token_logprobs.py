@@ -258,8 +258,8 @@ def test_results_do_not_depend_on_neighbours(ctx):
     logits, tokens = make(40, 30011, "bfloat16", 30)
     r = check(ctx, logits, tokens, 20)
     again = K.token_logprobs(ctx, logits, tokens, top=20)
-    for a, b in zip(r, again):
-        assert torch.equal(a, b)
+    for name in ("logprobs", "entropy", "lse", "row_max", "log_sum", "top_logprobs", "top_tokens"):
+        assert torch.equal(getattr(r, name), getattr(again, name))
     one = check(ctx, logits[7:8], tokens[7:8], 20)
     assert torch.equal(one.top_tokens[0], r.top_tokens[7])
 

@@ -39,5 +39,5 @@ def test_null_context():
     assert lib.tb_quantize_rows(None, 1, 1, None, 0, 1, None, 1, None) == _lib.TB_ERR_INVALID
     assert lib.tb_int8_gemm(None, 1, 1, 1, None, 16, None, None, 16, None, None, 4, None, 0, 1) == _lib.TB_ERR_INVALID
     assert lib.tb_int8_connected_fwd(None, 1, 1, 1, None, 0, 1, None, 16, None, None, 4, None, 0, 1) == _lib.TB_ERR_INVALID
-    assert lib.tb_token_logprobs_fwd(None, 1, 1, None, 0, 1, None, 1.0, 0, None, None, None, None, None) == _lib.TB_ERR_INVALID
-    assert lib.tb_token_logprobs_bwd(None, 1, 1, None, 0, 1, None, 1.0, None, None, None, None, None, 1) == _lib.TB_ERR_INVALID
+    assert lib.tb_token_logprobs_fwd(None, 1, 1, None, 0, 1, None, 1.0, 0, None, None, None, None, None, None, None) == _lib.TB_ERR_INVALID
+    assert lib.tb_token_logprobs_bwd(None, 1, 1, None, 0, 1, None, 1.0, None, None, None, None, None, None, 1) == _lib.TB_ERR_INVALID
