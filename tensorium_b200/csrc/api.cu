@@ -344,6 +344,7 @@ int tb_sync(tb_ctx* ctx) {
     TB_CHECK_CUDA(cudaMemcpy(&st, ctx->d_status, sizeof(int), cudaMemcpyDeviceToHost));
     if (st != 0) {
         cudaMemset(ctx->d_status, 0, sizeof(int));
+        cudaMemset(ctx->tile_cnt, 0, sizeof(int) * ctx->tile_cnt_len);  // a kernel that gave up leaves counts behind
         return fail(TB_ERR_DEVICE, "a kernel reported device status %d", st);
     }
     return TB_OK;

@@ -19,14 +19,10 @@ struct Int8Args {
     int64_t y_stride;
 };
 
-__device__ __forceinline__ float int8_epilogue(int acc, float scale, float bias, bool has_bias, int act) {
-    float v = __fmul_rn(__int2float_rn(acc), scale);
-    if (has_bias) v = __fadd_rn(v, bias);
-    return tb_activate_dev(v, act);
-}
-
-// tensor-core product (int8_tc.cu); after_quantize: the kernel before it on the stream is the one
-// that writes a and a_scales, and lets this one start early
-int int8_gemm_tc(tb_ctx* ctx, const Int8Args& p, int64_t y_type, bool after_quantize);
+// Tensor-core product (int8_tc.cu). after_quantize: the kernel before it on the stream is the one that
+// writes a and a_scales, and lets this one start early. scratch: the workspace is free from there on; where that is not its
+// start, int8_gemm_scratch more bytes have to be reserved.
+int int8_gemm_tc(tb_ctx* ctx, const Int8Args& p, int64_t y_type, bool after_quantize, size_t scratch);
+size_t int8_gemm_scratch(const tb_ctx* ctx, int64_t m);
 
 }  // namespace tbi

@@ -8,9 +8,10 @@
 // 128-byte swizzled rows; TMA fills zeros past k, m and n, so no size needs padding. int32 sums are
 // exact in any order, which is what lets k be split freely.
 //
-// k_int8_stream: one tile per CTA; a cluster of CTAs along k shares a tile when the tiles alone do
-// not fill the GPU, and sums its int32 partials through distributed shared memory, each CTA a part
-// of the tokens.
+// k_int8_stream: one CTA per SM on tiles of 128 channels x up to 128 tokens. Tiles that do not fill a wave of SMs are
+// shared out by k, to the byte evenly, since one SM streams from HBM at 43 GB/s at most (measured, with 5 as
+// with 10 stages in flight): only with equal shares do all of them together reach its rate. The CTAs of a tile leave
+// int32 sums in the workspace, and the last of them to finish adds them.
 // k_int8_pair: persistent CTA pairs (cta_group::2) on 256 x 256 tiles with two accumulators in
 // TMEM, so the epilogue of one tile runs under the products of the next.
 //
@@ -63,14 +64,6 @@ __device__ __forceinline__ void mma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_
             "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate));
 }
 
-__device__ __forceinline__ void st_cluster(unsigned local, unsigned rank, int v) {
-    unsigned remote;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(remote) : "r"(local), "r"(rank));
-    asm volatile("st.shared::cluster.s32 [%0], %1;\n" ::"r"(remote), "r"(v) : "memory");
-}
-
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory"); }
 // waits for the kernel before this one (and its writes) when launched with programmatic serialization
 __device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
 
@@ -111,148 +104,208 @@ template <typename T> struct Channel {
     }
 };
 
-constexpr int I8_MAX_STAGES = 8;
-constexpr int I8_STREAM_SMEM = 112 * 1024;  // two CTAs per SM
+// ---- one CTA on 128 channels x up to 128 tokens -----------------------------------------------------
+constexpr int I8S_MAX_STAGES = 12, I8S_THREADS = 320;
+constexpr int I8S_SMEM = 216 * 1024;
 
-template <typename T, int BT>
-__global__ void __launch_bounds__(192) k_int8_stream(const __grid_constant__ I8Maps maps, const Int8Args p, const int stages,
-                                                     int* status) {
-    constexpr int STAGE_BYTES = I8_W_BYTES + BT * I8_BK;
-    constexpr int COLS = BT < 32 ? 32 : BT;
+struct StreamArgs {
+    int bt;        // tokens of a tile: a multiple of 16 up to 128
+    int stages;
+    int tiles_m, ktiles;
+    int sk_tiles;  // tiles 0 .. sk_tiles - 1 are shared out by units of 128 bytes of k, the others whole
+    int dp_tiles;  // tiles after them
+    int* partial;  // [2 x CTA][bt / 4][128 channels][4 tokens]
+    int* counters; // per shared tile: CTAs that have left their sums, left at 0
+};
+
+// A CTA's work in order: its range of the shared tiles' units, then every gridDim.x-th whole tile.
+struct StreamWork {
+    int u, end, next, ktiles, tiles, step;
+    int tile, kb, ke;  // the current piece
+    __device__ StreamWork(const StreamArgs& a)
+        : u((int)((int64_t)a.sk_tiles * a.ktiles * blockIdx.x / gridDim.x)),
+          end((int)((int64_t)a.sk_tiles * a.ktiles * (blockIdx.x + 1) / gridDim.x)),
+          next(a.sk_tiles + blockIdx.x), ktiles(a.ktiles), tiles(a.sk_tiles + a.dp_tiles), step(gridDim.x) {}
+    __device__ __forceinline__ bool take() {
+        if (u < end) {
+            tile = u / ktiles;
+            kb = u - tile * ktiles;
+            ke = min(ktiles, kb + end - u);
+            u += ke - kb;
+            return true;
+        }
+        if (next >= tiles) return false;
+        tile = next, kb = 0, ke = ktiles;
+        next += step;
+        return true;
+    }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(I8S_THREADS, 1) k_int8_stream(const __grid_constant__ I8Maps maps, const Int8Args p, const StreamArgs g,
+                                                                 int* status) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     const unsigned sbase = ((unsigned)__cvta_generic_to_shared(smem_raw) + 1023u) & ~1023u;
-    __shared__ __align__(8) uint64_t full_bar[I8_MAX_STAGES], empty_bar[I8_MAX_STAGES], done_bar;
+    __shared__ __align__(8) uint64_t full_bar[I8S_MAX_STAGES], empty_bar[I8S_MAX_STAGES], tfull_bar[2], tempty_bar[2], drain_bar;
     __shared__ uint32_t tmem_base;
     __shared__ volatile int abort_flag;
-    __shared__ __align__(16) float a_scales[BT];
+    __shared__ int last;
+    __shared__ __align__(16) float a_scales[2][128];
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int splits = gridDim.z, z = blockIdx.z;
-    const int64_t n0 = (int64_t)blockIdx.x * 128, m0 = (int64_t)blockIdx.y * BT;
-    const int ktiles = (int)((p.k + I8_BK - 1) / I8_BK);
-    const int kb = (int)((int64_t)ktiles * z / splits), ke = (int)((int64_t)ktiles * (z + 1) / splits);
+    const int bt = g.bt, stages = g.stages;
+    const int stage_bytes = I8_W_BYTES + bt * I8_BK;
 
+    int pre = 0;
     if (tid == 0) {
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<uint64_t>(&maps.w)) : "memory");
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<uint64_t>(&maps.a)) : "memory");
         for (int s = 0; s < stages; ++s) {
             tc::mbar_init(&full_bar[s], 1);
             tc::mbar_init(&empty_bar[s], 1);
         }
-        tc::mbar_init(&done_bar, 1);
+        for (int b = 0; b < 2; ++b) {
+            tc::mbar_init(&tfull_bar[b], 1);
+            tc::mbar_init(&tempty_bar[b], 8);  // one arrival per epilogue warp
+        }
+        tc::mbar_init(&drain_bar, 1);
         abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+        // the first stages' weights at once: they do not depend on the kernel before
+        for (StreamWork w(g); pre < stages && w.take();)
+            for (int kt = w.kb; kt < w.ke && pre < stages; ++kt, ++pre) {
+                tc::mbar_arrive_expect_tx(&full_bar[pre], stage_bytes);
+                tc::tma_load_2d(sbase + pre * stage_bytes, &maps.w, &full_bar[pre], kt * I8_BK, w.tile / g.tiles_m * 128);
+            }
     }
-    if (warp == 1) tc::tmem_alloc(&tmem_base, COLS);
+    if (warp == 1) tc::tmem_alloc(&tmem_base, 256);
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
-    if (splits > 1) cluster_arrive();  // waited for before the first remote store: every CTA has started
     const uint32_t tmem0 = tmem_base;
 
     if (warp == 0) {
         if (lane == 0) {
-            // weights of the first stages before the tokens: they do not depend on the kernel before
-            const int pre = min(stages, ke - kb);
-            for (int j = 0; j < pre; ++j) {
-                tc::mbar_arrive_expect_tx(&full_bar[j], STAGE_BYTES);
-                tc::tma_load_2d(sbase + j * STAGE_BYTES, &maps.w, &full_bar[j], (kb + j) * I8_BK, (int)n0);
-            }
             grid_dep_wait();
-            int j = 0;
-            for (; j < ke - kb; ++j) {
-                const int st = j % stages, use = j / stages;
-                const unsigned sw = sbase + st * STAGE_BYTES;
-                if (use > 0) {
-                    if (!tc::mbar_wait_bounded(&empty_bar[st], (use - 1) & 1, &abort_flag, status, 931)) break;
-                    tc::mbar_arrive_expect_tx(&full_bar[st], STAGE_BYTES);
-                    tc::tma_load_2d(sw, &maps.w, &full_bar[st], (kb + j) * I8_BK, (int)n0);
+            int it = 0, st = 0, ph = 1;  // ph: parity of the stage's last release
+            bool ok = true;
+            for (StreamWork w(g); ok && w.take();) {
+                const int w_row = w.tile / g.tiles_m * 128, a_row = w.tile % g.tiles_m * bt;
+                for (int kt = w.kb; kt < w.ke; ++kt, ++it) {
+                    const unsigned sw = sbase + st * stage_bytes;
+                    if (it >= pre) {
+                        if (!tc::mbar_wait_bounded(&empty_bar[st], ph, &abort_flag, status, 931)) {
+                            ok = false;
+                            break;
+                        }
+                        tc::mbar_arrive_expect_tx(&full_bar[st], stage_bytes);
+                        tc::tma_load_2d(sw, &maps.w, &full_bar[st], kt * I8_BK, w_row);
+                    }
+                    tc::tma_load_2d(sw + I8_W_BYTES, &maps.a, &full_bar[st], kt * I8_BK, a_row);
+                    if (++st == stages) st = 0, ph ^= 1;
                 }
-                tc::tma_load_2d(sw + I8_W_BYTES, &maps.a, &full_bar[st], (kb + j) * I8_BK, (int)m0);
             }
             // the copies land before the CTA ends, after an abort too: the last use of every stage
-            for (int i = max(0, j - stages); i < j; ++i) tc::mbar_wait_limit(&full_bar[i % stages], (i / stages) & 1);
+            for (int i = max(0, it - stages); i < it; ++i) tc::mbar_wait_limit(&full_bar[i % stages], (i / stages) & 1);
         }
         __syncwarp();
     } else if (warp == 1) {
         if (lane == 0) {
-            bool issued = false;
-            for (int j = 0; j < ke - kb; ++j) {
-                const int st = j % stages, use = j / stages;
-                if (!tc::mbar_wait_bounded(&full_bar[st], use & 1, &abort_flag, status, 932)) break;
+            const uint32_t idesc = idesc_i8(128, bt);
+            int st = 0, ph = 0, n = 0;
+            bool ok = true, issued = false;
+            for (StreamWork w(g); ok && w.take(); ++n) {
+                const int buf = n & 1, u = n >> 1;
+                if (u > 0 && !tc::mbar_wait_bounded(&tempty_bar[buf], (u - 1) & 1, &abort_flag, status, 932)) break;
                 tc::tc_fence_after();
-                const unsigned sw = sbase + st * STAGE_BYTES;
+                const uint32_t d = tmem0 + buf * 128;
+                for (int kt = w.kb; kt < w.ke; ++kt) {
+                    if (!tc::mbar_wait_bounded(&full_bar[st], ph, &abort_flag, status, 933)) {
+                        ok = false;
+                        break;
+                    }
+                    tc::tc_fence_after();
+                    const unsigned sw = sbase + st * stage_bytes;
 #pragma unroll
-                for (int kk = 0; kk < I8_BK / 32; ++kk)
-                    mma_i8<1>(tmem0, desc_k_sw128(sw + kk * 32), desc_k_sw128(sw + I8_W_BYTES + kk * 32), idesc_i8(128, BT),
-                              (j || kk) ? 1u : 0u);
-                issued = true;
-                tc::mma_commit(&empty_bar[st]);
+                    for (int kk = 0; kk < I8_BK / 32; ++kk)
+                        mma_i8<1>(d, desc_k_sw128(sw + kk * 32), desc_k_sw128(sw + I8_W_BYTES + kk * 32), idesc, (kt > w.kb || kk) ? 1u : 0u);
+                    issued = true;
+                    tc::mma_commit(&empty_bar[st]);
+                    if (++st == stages) st = 0, ph ^= 1;
+                }
+                if (ok) tc::mma_commit(&tfull_bar[buf]);
             }
-            if (issued) {  // also after an abort: no MMA runs on when TMEM is freed
-                tc::mma_commit(&done_bar);
-                tc::mbar_wait_limit(&done_bar, 0);
+            if (issued) {  // every MMA has finished before TMEM is freed
+                tc::mma_commit(&drain_bar);
+                tc::mbar_wait_limit(&drain_bar, 0);
             }
         }
         __syncwarp();
-    }
-    const int quarter = warp & 3, ch = quarter * 32 + lane;
-    const uint32_t taddr = tmem0 + ((uint32_t)(quarter * 32) << 16);
-    bool ok = true;
-    if (warp >= 2) {
-        grid_dep_wait();
-        for (int i = ch; i < BT; i += 128) a_scales[i] = m0 + i < p.m ? p.a_scales[m0 + i] : 0.f;
-        asm volatile("bar.sync 1, 128;\n" ::: "memory");
-        ok = tc::mbar_wait_bounded(&done_bar, 0, &abort_flag, status, 933);
-        ok = __all_sync(0xffffffffu, ok && !abort_flag);
-        tc::tc_fence_after();
-    }
-    if (splits == 1) {
-        if (warp >= 2 && ok) {
-            const Channel<T> c(p, n0 + ch);
-#pragma unroll 1
-            for (int c0 = 0; c0 < BT; c0 += 16) {
-                uint32_t r[16];
-                tc::tmem_ld16_issue(taddr + c0, r);
-                tc::tmem_wait16(r);
-                c.template store<16>(p, m0 + c0, a_scales + c0, reinterpret_cast<int*>(r));
-            }
-        }
     } else {
-        // each CTA of the cluster sums its share of the tile's tokens: [source][token][channel] in its
-        // own buffer behind the stages, filled by every CTA
-        const int share = BT / splits;
-        const unsigned red = sbase + stages * STAGE_BYTES;
-        cluster_wait();
-        if (warp >= 2 && ok) {
+        grid_dep_wait();  // a_scales
+        const int quarter = warp & 3, half = (warp - 2) >> 2, ch = quarter * 32 + lane, et = tid - 64;
+        const int64_t units = (int64_t)g.sk_tiles * g.ktiles;
+        int n = 0;
+        for (StreamWork w(g); w.take(); ++n) {
+            const int buf = n & 1, u = n >> 1;
+            const int64_t m0 = (int64_t)(w.tile % g.tiles_m) * bt;
+            if (et < bt) a_scales[buf][et] = m0 + et < p.m ? p.a_scales[m0 + et] : 0.f;
+            const Channel<T> c(p, (int64_t)(w.tile / g.tiles_m) * 128 + ch);
+            const bool ok = !abort_flag && tc::mbar_wait_bounded(&tfull_bar[buf], u & 1, &abort_flag, status, 934);
+            if (tc::epi_any(!ok)) break;  // tcgen05.ld is warp-collective: the epilogue warps leave together
+            tc::tc_fence_after();
+            const uint32_t taddr = tmem0 + buf * 128 + ((uint32_t)(quarter * 32) << 16);
+            const bool whole = w.kb == 0 && w.ke == g.ktiles;
+            // this CTA's sums of a shared tile: slot 0 where its piece begins inside the tile, 1 where it ends there
+            int4* slot = reinterpret_cast<int4*>(g.partial) + (int64_t)(2 * blockIdx.x + (w.kb == 0)) * bt * 32 + ch;
 #pragma unroll 1
-            for (int c0 = 0; c0 < BT; c0 += 16) {
+            for (int c0 = half * 16; c0 < bt; c0 += 32) {
                 uint32_t r[16];
                 tc::tmem_ld16_issue(taddr + c0, r);
                 tc::tmem_wait16(r);
+                if (whole) {
+                    c.template store<16>(p, m0 + c0, a_scales[buf] + c0, reinterpret_cast<int*>(r));
+                } else {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int c = c0 + i, to = c / share;
-                    st_cluster(red + ((z * share + c - to * share) * 128 + ch) * 4, to, (int)r[i]);
+                    for (int i = 0; i < 4; ++i)
+                        __stcg(slot + (c0 / 4 + i) * 128, make_int4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]));
                 }
             }
-        }
-        __syncwarp();
-        cluster_arrive();
-        cluster_wait();
-        if (warp >= 2 && ok) {
-            const Channel<T> c(p, n0 + ch);
-            const int* buf = reinterpret_cast<const int*>(smem_raw + (red - (unsigned)__cvta_generic_to_shared(smem_raw))) + ch;
-            for (int i = 0; i < share; i += 2) {  // shares are powers of two from 2 on
-                int acc[2] = {0, 0};
-#pragma unroll 4
-                for (int s = 0; s < splits; ++s)
-                    for (int u = 0; u < 2; ++u) acc[u] += buf[(s * share + i + u) * 128];
-                c.template store<2>(p, m0 + z * share + i, a_scales + z * share + i, acc);
+            tc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&tempty_bar[buf]);
+            if (whole) continue;
+            // the last of the tile's CTAs to get here adds their sums (int32: the same in any order)
+            const int64_t u0 = (int64_t)w.tile * g.ktiles;
+            const int first = (int)(((u0 + 1) * gridDim.x - 1) / units), end = (int)(((u0 + g.ktiles) * gridDim.x - 1) / units) + 1;
+            __threadfence();
+            tc::epi_sync();
+            if (et == 0) {
+                last = atomicAdd(&g.counters[w.tile], 1) == end - first - 1;
+                if (last) g.counters[w.tile] = 0;  // ready for the next launch
+            }
+            tc::epi_sync();
+            if (!last) continue;
+            __threadfence();
+#pragma unroll 1
+            for (int c0 = half * 16; c0 < bt; c0 += 32) {
+                int r[16] = {};
+#pragma unroll 2
+                for (int j = first; j < end; ++j) {
+                    const int4* q = reinterpret_cast<const int4*>(g.partial) + (int64_t)(2 * j + (j == first)) * bt * 32 + ch;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int4 v = __ldcg(q + (c0 / 4 + i) * 128);
+                        r[4 * i] += v.x, r[4 * i + 1] += v.y, r[4 * i + 2] += v.z, r[4 * i + 3] += v.w;
+                    }
+                }
+                c.template store<16>(p, m0 + c0, a_scales[buf] + c0, r);
             }
         }
     }
     tc::tc_fence_before();
     __syncthreads();
-    if (warp == 1) tc::tmem_dealloc(tmem0, COLS);
+    if (warp == 1) tc::tmem_dealloc(tmem0, 256);
 }
 
 // ---- CTA pairs ----------------------------------------------------------------------------------
@@ -467,20 +520,43 @@ int launch_cluster(tb_ctx* ctx, const char* what, dim3 grid, int threads, int sm
     return check_launch(what);
 }
 
-template <int BT> int launch_stream(tb_ctx* ctx, const Int8Args& p, int64_t y_type, bool early, int splits) {
-    constexpr int stage = I8_W_BYTES + BT * I8_BK;
+// `scratch`: where the workspace is free
+int launch_stream(tb_ctx* ctx, const Int8Args& p, int64_t y_type, bool early, int bt, size_t scratch) {
     I8Maps maps;
     int r = encode_rows(&maps.w, p.w, p.k, p.n, p.w_stride, 128);
-    if (r == TB_OK) r = encode_rows(&maps.a, p.a, p.k, p.m, p.a_stride, BT);
+    if (r == TB_OK) r = encode_rows(&maps.a, p.a, p.k, p.m, p.a_stride, bt);
     if (r != TB_OK) return r;
-    // two CTAs per SM, so that one's set-up and epilogue run under the other's products
-    const int red = splits > 1 ? BT * 512 : 0;
-    const int stages = std::min<int>(I8_MAX_STAGES, (I8_STREAM_SMEM - 1024 - red) / stage);
-    const int smem = stages * stage + red + 1024;
-    const dim3 grid((unsigned)ceil_div(p.n, 128), (unsigned)ceil_div(p.m, BT), (unsigned)splits);
+    const int64_t tiles_m = ceil_div(p.m, bt), tiles = tiles_m * ceil_div(p.n, 128), ktiles = ceil_div(p.k, I8_BK), sms = ctx->sm_count;
+    StreamArgs g = {};
+    g.bt = bt;
+    g.stages = (int)std::min<int64_t>(I8S_MAX_STAGES, (I8S_SMEM - 1024) / (I8_W_BYTES + bt * I8_BK));
+    g.tiles_m = (int)tiles_m;
+    g.ktiles = (int)ktiles;
+    // Whole tiles in full waves; what is left of one wave, with the wave before it, is shared out evenly (in
+    // pieces of 4 units at least on average) where that saves more than leaving and adding the partial sums costs: 4 us, in
+    // which an SM loads 40 bytes a nanosecond.
+    int64_t grid = std::min(tiles, sms);
+    if (tiles % sms != 0) {
+        const int64_t sk = tiles < sms ? tiles : tiles % sms + sms, unit = I8_W_BYTES + bt * I8_BK;
+        const int64_t sk_grid = std::min(sms, ceil_div(sk * ktiles, 4));
+        const double whole = (double)ceil_div(sk, sms) * ktiles * unit / 40, shared = (double)sk * ktiles * unit / sk_grid / 40 + 4000;
+        if (sk_grid > std::min(tiles, sms) - (tiles > sms) && shared < whole) {
+            g.sk_tiles = (int)sk;
+            grid = sk_grid;
+        }
+    }
+    g.dp_tiles = (int)(tiles - g.sk_tiles);
+    if (g.sk_tiles) {
+        const size_t need = scratch + (size_t)grid * 2 * bt * 128 * 4;
+        if (need > ctx->ws_bytes && scratch) return fail(TB_ERR_STATE, "int8 product: workspace not reserved");
+        if ((r = ensure_workspace(ctx, need)) != TB_OK) return r;
+        g.partial = reinterpret_cast<int*>(static_cast<char*>(ctx->ws) + scratch);
+        g.counters = ctx->tile_cnt;
+    }
+    const int smem = g.stages * (I8_W_BYTES + bt * I8_BK) + 1024;
     return elem_dispatch(y_type, [&](auto t) {
-        return launch_cluster<k_int8_stream<decltype(t), BT>>(ctx, "k_int8_stream", grid, 192, smem, I8_STREAM_SMEM,
-                                                              dim3(1, 1, (unsigned)splits), early, maps, p, stages, ctx->d_status);
+        return launch_cluster<k_int8_stream<decltype(t)>>(ctx, "k_int8_stream", dim3((unsigned)grid), I8S_THREADS, smem, I8S_SMEM, dim3(1, 1, 1),
+                                                          early, maps, p, g, ctx->d_status);
     });
 }
 
@@ -499,22 +575,18 @@ int launch_pair(tb_ctx* ctx, const Int8Args& p, int64_t y_type, bool early) {
 
 }  // namespace
 
-int int8_gemm_tc(tb_ctx* ctx, const Int8Args& p, int64_t y_type, bool early) {
+// Tokens of a tile of the single-CTA kernel: up to 128 in as many equal tiles as it takes.
+static int stream_tokens(int64_t m) { return (int)round_up(ceil_div(m, ceil_div(m, 128)), 16); }
+
+size_t int8_gemm_scratch(const tb_ctx* ctx, int64_t m) { return (size_t)ctx->sm_count * 2 * stream_tokens(m) * 128 * 4; }
+
+int int8_gemm_tc(tb_ctx* ctx, const Int8Args& p, int64_t y_type, bool early, size_t scratch) {
     const int64_t sms = ctx->sm_count;
     // pairs once their tiles occupy two thirds of the SMs
-    if (p.m > 128 && ceil_div(p.m, 256) * ceil_div(p.n, 256) * 2 * 3 >= sms * 2) return launch_pair(ctx, p, y_type, early);
-    const int bt = p.m <= 16 ? 16 : p.m <= 32 ? 32 : p.m <= 64 ? 64 : 128;
-    if (ceil_div(p.m, bt) > 65535) return launch_pair(ctx, p, y_type, early);
-    const int64_t tiles = ceil_div(p.n, 128) * ceil_div(p.m, bt), ktiles = ceil_div(p.k, I8_BK);
-    // k in up to 8 parts while there are fewer CTAs than two per SM, parts of 4 stages at least
-    int splits = 1;
-    while (splits < 8 && splits * 2 <= bt && tiles * splits * 2 <= sms * 2 && ktiles >= splits * 2 * 4) splits *= 2;
-    switch (bt) {
-    case 16: return launch_stream<16>(ctx, p, y_type, early, splits);
-    case 32: return launch_stream<32>(ctx, p, y_type, early, splits);
-    case 64: return launch_stream<64>(ctx, p, y_type, early, splits);
-    default: return launch_stream<128>(ctx, p, y_type, early, splits);
-    }
+    const int64_t tiles = ceil_div(p.m, 128) * ceil_div(p.n, 128);
+    if ((p.m > 128 && ceil_div(p.m, 256) * ceil_div(p.n, 256) * 2 * 3 >= sms * 2) || tiles * ceil_div(p.k, I8_BK) >= ((int64_t)1 << 30))
+        return launch_pair(ctx, p, y_type, early);
+    return launch_stream(ctx, p, y_type, early, stream_tokens(p.m), scratch);
 }
 
 }  // namespace tbi
