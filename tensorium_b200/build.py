@@ -2,8 +2,8 @@
 
 Every ``csrc/*.cu`` file is compiled by nvcc for sm_100a only (the reference instead JIT-compiles
 one generic .cu string with NVRTC at start-up, source/nncuda.pas:1586-1642) and linked into one
-shared library with a plain C ABI (include/tensorium_b200.h).  The library is built in-tree so it
-travels with the repository snapshot.
+shared library with a plain C ABI (include/tensorium_b200.h); ``bind/tokens_fast.cpp`` becomes a small
+Python extension over it.  Both are built in-tree so they travel with the repository snapshot.
 
     python -m tensorium_b200.build [--force] [-j N] [-v]
 """
@@ -22,6 +22,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 OBJ = PKG / "_build"
 LIB = PKG / "libtensorium_b200.so"
+FAST_SRC = PKG / "bind" / "tokens_fast.cpp"
+FAST = PKG / "_tokens_fast.so"  # Python extension over the library (see its source)
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 # --fmad=false: no silent a*b+c contraction; every FMA on the path is an explicit fmaf, so the
@@ -67,6 +69,25 @@ def _compile(src: Path, verbose: bool, extra) -> Path:
     return obj
 
 
+def _build_fast(force: bool, verbose: bool) -> None:
+    if not force and not _stale(FAST, [FAST_SRC, LIB]):
+        return
+    import sysconfig
+
+    import torch
+    t = Path(torch.__file__).resolve().parent
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I", str(t / "include"), "-I", str(t / "include" / "torch" / "csrc" / "api" / "include"),
+           "-I", sysconfig.get_paths()["include"], "-I", str(Path(nvcc()).resolve().parent.parent / "include"), str(FAST_SRC), "-o", str(FAST),
+           "-L", str(t / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-L", str(PKG), f"-l:{LIB.name}",
+           "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on {FAST_SRC.name}:\n{r.stdout}\n{r.stderr}")
+
+
 def build(force: bool = False, jobs: int | None = None, verbose: bool = False, extra=()) -> Path:
     OBJ.mkdir(exist_ok=True)
     srcs = _sources()
@@ -83,6 +104,7 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False, e
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    _build_fast(force, verbose)
     return LIB
 
 

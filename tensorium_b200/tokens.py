@@ -20,6 +20,11 @@ import torch
 from ._lib import ACT, BF16_ELEM, F16_ELEM, F32_ELEM, check, lib
 from .context import Context
 
+try:
+    from . import _tokens_fast as _fast  # ordinary calls, checked and allocated outside Python
+except ImportError as e:
+    raise ImportError(f"{e}: build it with `python -m tensorium_b200.build`") from e
+
 _current_stream = torch._C._cuda_getCurrentRawStream
 _ELEM = {torch.float32: F32_ELEM, torch.bfloat16: BF16_ELEM, torch.float16: F16_ELEM}
 
@@ -159,6 +164,10 @@ def int8_product(ctx: Context, a, a_scales, w, w_scales, bias=None, activation="
 def int8_connected(ctx: Context, x, w, w_scales, bias=None, activation="linear", dtype=None, out=None):
     """The connected layer on int8 weights: every row of x [tokens, k] is quantized on the way in
     (quantize_rows) and multiplied with w [channels, k] (int8_product). dtype: x's unless given."""
+    if dtype is None and out is None:
+        y = _fast.int8_connected(ctx.handle.value, ctx.device, ctx.raw_stream, x, w, w_scales, bias, ACT.get(activation, activation))
+        if y is not None:
+            return y if y.__class__ is not int else check(y)
     m, k, x_stride = _matrix(ctx, x, "x", _ELEM)
     n, kw, w_stride = _matrix(ctx, w, "w", _INT8)
     if k != kw:
@@ -180,6 +189,9 @@ def token_logprobs(ctx: Context, logits, tokens=None, top: int = 0, temperature:
     """Of the softmax of logits / temperature, logits [rows, vocab]: the log probability of tokens
     (int64 [rows]; negative: none given, 0), the entropy, the log of the sum of exponentials and, with
     top > 0 (at most 32), the most probable tokens in descending order (equal logits: the lowest first)."""
+    r = _fast.token_logprobs(ctx.handle.value, ctx.device, ctx.raw_stream, logits, tokens, top, temperature)
+    if r is not None:
+        return TokenLogprobs(r[0], tokens is not None, r[1], r[2]) if r.__class__ is tuple else check(r)
     rows, vocab, stride = _matrix(ctx, logits, "logits", _ELEM)
     t = None if tokens is None else _vector(ctx, tokens, "tokens", torch.int64, rows)
     if top > 0:
@@ -199,6 +211,11 @@ def token_logprobs_backward(ctx: Context, logits, tokens, forward: TokenLogprobs
     """Gradient with respect to the logits of sum(grad_logprobs * logprobs + grad_entropy * entropy),
     from token_logprobs' results on the same logits, tokens and temperature (float32 gradients, a row
     each; None: 0). out may be the logits themselves."""
+    if out is None:
+        d = _fast.token_logprobs_backward(ctx.handle.value, ctx.device, ctx.raw_stream, logits, tokens, forward.stats,
+                                          grad_logprobs, grad_entropy, temperature)
+        if d is not None:
+            return d if d.__class__ is not int else check(d)
     rows, vocab, stride = _matrix(ctx, logits, "logits", _ELEM)
     if grad_logprobs is not None and tokens is None:
         raise ValueError("grad_logprobs without tokens")

@@ -1,4 +1,5 @@
 """What the token operators' Python entry points refuse before they reach a GPU."""
+import ctypes
 import types
 
 import pytest
@@ -7,7 +8,7 @@ import torch
 from tensorium_b200 import _lib
 from tensorium_b200 import tokens as K
 
-CTX = types.SimpleNamespace(device=0)
+CTX = types.SimpleNamespace(device=0, handle=ctypes.c_void_p(), raw_stream=0)  # a closed context
 
 
 def test_tensors_that_are_not_on_the_gpu():
