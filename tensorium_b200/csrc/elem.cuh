@@ -31,6 +31,18 @@ template <typename T> struct __align__(16) Vec {
 inline bool elem_type_ok(int64_t t) { return t == TB_F32 || t == TB_BF16 || t == TB_F16; }
 inline size_t elem_size(int64_t t) { return t == TB_F32 ? 4 : 2; }
 
+// launch() that lets the kernel be scheduled while the one before it on the stream still runs: its set-up hides the
+// launch's latency, and it waits for that kernel's end itself (TB_GRID_DEP_ENTRY) before it reads or writes
+// global memory.
+template <typename... KArgs, typename... Args>
+int launch_early(tb_ctx* ctx, const char* what, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, Args&&... args) {
+    const int pdl = ctx->pdl;
+    ctx->pdl = 1;
+    const int r = launch(ctx, what, kernel, grid, block, smem, std::forward<Args>(args)...);
+    ctx->pdl = pdl;
+    return r;
+}
+
 // f(T()) for the element type t
 template <typename F> int elem_dispatch(int64_t t, F&& f) {
     if (t == TB_F32) return f(float());

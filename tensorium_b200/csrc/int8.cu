@@ -141,14 +141,14 @@ int quantize_rows(tb_ctx* ctx, int64_t rows, int64_t cols, const void* x, int64_
         const T* xt = static_cast<const T*>(x);
         if (vecs <= 128) {
             const unsigned grid = (unsigned)ceil_div(rows, 4);
-            return vec ? launch(ctx, "k_quantize_rows", k_quantize_rows<T, true, true>, dim3(grid), dim3(128), 0, rows, cols, xt, x_stride, codes, code_stride, scales, code_vec)
-                       : launch(ctx, "k_quantize_rows", k_quantize_rows<T, false, true>, dim3(grid), dim3(128), 0, rows, cols, xt, x_stride, codes, code_stride, scales, code_vec);
+            return vec ? launch_early(ctx, "k_quantize_rows", k_quantize_rows<T, true, true>, dim3(grid), dim3(128), 0, rows, cols, xt, x_stride, codes, code_stride, scales, code_vec)
+                       : launch_early(ctx, "k_quantize_rows", k_quantize_rows<T, false, true>, dim3(grid), dim3(128), 0, rows, cols, xt, x_stride, codes, code_stride, scales, code_vec);
         }
         // 64 bytes a thread where there are rows enough to fill the GPU, 16 where a row's latency counts
         const int64_t per = rows >= 4 * ctx->sm_count ? 4 : 1;
         const unsigned threads = (unsigned)std::min<int64_t>(1024, round_up(ceil_div(vecs, per), 32));
-        return vec ? launch(ctx, "k_quantize_rows", k_quantize_rows<T, true, false>, dim3((unsigned)rows), dim3(threads), 0, rows, cols, xt, x_stride, codes, code_stride, scales, code_vec)
-                   : launch(ctx, "k_quantize_rows", k_quantize_rows<T, false, false>, dim3((unsigned)rows), dim3(threads), 0, rows, cols, xt, x_stride, codes, code_stride, scales, code_vec);
+        return vec ? launch_early(ctx, "k_quantize_rows", k_quantize_rows<T, true, false>, dim3((unsigned)rows), dim3(threads), 0, rows, cols, xt, x_stride, codes, code_stride, scales, code_vec)
+                   : launch_early(ctx, "k_quantize_rows", k_quantize_rows<T, false, false>, dim3((unsigned)rows), dim3(threads), 0, rows, cols, xt, x_stride, codes, code_stride, scales, code_vec);
     });
 }
 
@@ -355,7 +355,7 @@ template <typename T, bool VEC, int B8> int launch_few_b(tb_ctx* ctx, const FewA
     a.kw = FEW_WARPS;
     while (a.kw > 1 && steps < a.kw * 4 && groups >= (int64_t)ctx->sm_count * (FEW_WARPS / a.kw) * 2) a.kw /= 2;
     const int64_t grid = std::min<int64_t>(ceil_div(groups, FEW_WARPS / a.kw), ctx->sm_count);
-    return launch(ctx, "k_int8_few", k_int8_few<T, VEC, B8>, dim3((unsigned)grid), dim3(FEW_THREADS),
+    return launch_early(ctx, "k_int8_few", k_int8_few<T, VEC, B8>, dim3((unsigned)grid), dim3(FEW_THREADS),
                   (size_t)(FEW_RING_BYTES + g.p.m * few_pitch(g.p.k)), a);
 }
 

@@ -655,10 +655,10 @@ template <typename T> int launch_logprobs(tb_ctx* ctx, LogprobArgs p) {
     }
     const dim3 grid((unsigned)(nw == 1 ? ceil_div(p.rows, 4) : p.rows * p.splits)), block((unsigned)(nw == 1 ? 128 : nw * 32));
     switch (nw) {
-    case 1: return launch(ctx, "k_token_logprobs", k_token_logprobs<T, 1>, grid, block, 0, p);
-    case 2: return launch(ctx, "k_token_logprobs", k_token_logprobs<T, 2>, grid, block, 0, p);
-    case 4: return launch(ctx, "k_token_logprobs", k_token_logprobs<T, 4>, grid, block, 0, p);
-    default: return launch(ctx, "k_token_logprobs", k_token_logprobs<T, 8>, grid, block, 0, p);
+    case 1: return launch_early(ctx, "k_token_logprobs", k_token_logprobs<T, 1>, grid, block, 0, p);
+    case 2: return launch_early(ctx, "k_token_logprobs", k_token_logprobs<T, 2>, grid, block, 0, p);
+    case 4: return launch_early(ctx, "k_token_logprobs", k_token_logprobs<T, 4>, grid, block, 0, p);
+    default: return launch_early(ctx, "k_token_logprobs", k_token_logprobs<T, 8>, grid, block, 0, p);
     }
 }
 
@@ -749,10 +749,10 @@ template <typename T> int launch_bwd(tb_ctx* ctx, LogprobBwdArgs p) {
     constexpr int E = 16 / sizeof(T);
     const int64_t chunks = ceil_div(p.vocab, E) + 1;  // one more where a row starts inside a chunk
     if (chunks <= 32 * 4)
-        return launch(ctx, "k_token_logprobs_bwd", k_token_logprobs_bwd<T, true>, dim3((unsigned)ceil_div(p.rows, 8)), dim3(256), 0, p);
+        return launch_early(ctx, "k_token_logprobs_bwd", k_token_logprobs_bwd<T, true>, dim3((unsigned)ceil_div(p.rows, 8)), dim3(256), 0, p);
     p.parts = ceil_div(chunks, 256 * 4);
     if (p.rows * p.parts > 2147483647) return fail(TB_ERR_UNSUPPORTED, "token logprobs: more than 2^31 parts of rows");
-    return launch(ctx, "k_token_logprobs_bwd", k_token_logprobs_bwd<T, false>, dim3((unsigned)(p.rows * p.parts)), dim3(256), 0, p);
+    return launch_early(ctx, "k_token_logprobs_bwd", k_token_logprobs_bwd<T, false>, dim3((unsigned)(p.rows * p.parts)), dim3(256), 0, p);
 }
 
 int check_logits(int64_t rows, int64_t vocab, const void* logits, int64_t type, int64_t stride, float temperature) {
