@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <cstring>
+#include <type_traits>
 
 namespace tbi {
 namespace {
@@ -27,6 +28,7 @@ struct LogprobArgs {
     float* log_sum;
     float* top_logprob;
     int64_t* top_token;
+    int steps;             // most steps of a part
     int splits;            // parts of a row, joined by the last of their CTAs to finish
     Part* parts;
     int* counters;         // finished parts of each row, left at 0
@@ -448,13 +450,12 @@ __device__ __forceinline__ void take(unsigned long long& list, unsigned long lon
 // pass only the groups that can hold one of the best are read again: those whose maximum reaches the k-th
 // largest of the threads' maxima, about k of them.
 constexpr int LP_U = 4;
-template <typename T> constexpr int LP_STEPS = sizeof(T) == 4 ? 16 : 32;  // most steps of a part
+// most steps of a part: 32 KB of groups to a CTA, and what an SM's threads share (float: 45 and 30)
+template <typename T> int lp_steps(int nw) { return nw == 8 ? (sizeof(T) == 4 ? 28 : 32) : (sizeof(T) == 4 ? 40 : 64); }
 
 constexpr int KEYS = 64;  // candidates that are ranked against one another
 
-template <typename T, int NW> struct RowShared {
-    T group_max[LP_STEPS<T>][NW * 32];
-    uint16_t queue[LP_STEPS<T> * NW * 32];
+template <int NW> struct RowShared {
     unsigned long long keys[NW][32];
     Sums sums[NW];
     unsigned long long found[KEYS], ranked[32];
@@ -467,11 +468,15 @@ template <int NW> __device__ __forceinline__ void row_sync() {
     else __syncthreads();
 }
 
-template <typename T, int NW> __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? 8 : 32 / NW) k_token_logprobs(const LogprobArgs p) {
+template <typename T, int NW, bool AHEAD>
+__global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? (AHEAD ? 6 : 8) : (AHEAD ? 24 : 32) / NW) k_token_logprobs(const LogprobArgs p) {
     TB_GRID_DEP_ENTRY();
     constexpr int E = 16 / sizeof(T), U = LP_U, NT = NW * 32, ROWS = NW == 1 ? 4 : 1;
-    __shared__ RowShared<T, NW> shared[ROWS];
-    RowShared<T, NW>& sh = shared[NW == 1 ? threadIdx.x >> 5 : 0];
+    __shared__ RowShared<NW> shared[ROWS];
+    extern __shared__ __align__(16) unsigned char dyn[];  // with top > 0: each row's group maxima, then its queue of groups
+    RowShared<NW>& sh = shared[NW == 1 ? threadIdx.x >> 5 : 0];
+    T (*const group_max)[NT] = reinterpret_cast<T (*)[NT]>(dyn + (NW == 1 ? threadIdx.x >> 5 : 0) * p.steps * NT * (sizeof(T) + 2));
+    uint16_t* const queue = reinterpret_cast<uint16_t*>(group_max + p.steps);
 
     const int lane = threadIdx.x & 31, warp = NW == 1 ? 0 : threadIdx.x >> 5, tid = warp * 32 + lane;
     const int64_t unit = NW == 1 ? (int64_t)blockIdx.x * ROWS + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
@@ -492,10 +497,21 @@ template <typename T, int NW> __global__ void __launch_bounds__(NW == 1 ? 128 : 
     int steps = 0;
     bool clamp = false;
     uint4 raw[U];
+    [[maybe_unused]] uint4 next[U];
+    [[maybe_unused]] bool next_whole = false;
+    if (AHEAD) next_whole = r.step(next, begin, tid, NT, stop);
     for (int v0 = begin; v0 < stop; v0 += NT * U, ++steps) {
-        const bool whole = r.step(raw, v0, tid, NT, stop);
+        bool whole;
+        if constexpr (AHEAD) {  // the next step's loads run under this step's sums
+#pragma unroll
+            for (int u = 0; u < U; ++u) raw[u] = next[u];
+            whole = next_whole;
+            if (v0 + NT * U < stop) next_whole = r.step(next, v0 + NT * U, tid, NT, stop);
+        } else {
+            whole = r.step(raw, v0, tid, NT, stop);
+        }
         const float m = Chunk<T>::vmax(raw);
-        if (p.top) sh.group_max[steps][tid] = Elem<T>::put(m);  // exact: m is one of the logits
+        if (p.top) group_max[steps][tid] = Elem<T>::put(m);  // exact: m is one of the logits
         a.raise(m, c, margin);
         a.template step<T>(raw, (stop - v0 + NT - 1) / NT, c, !whole, clamp);
     }
@@ -520,7 +536,7 @@ template <typename T, int NW> __global__ void __launch_bounds__(NW == 1 ? 128 : 
         const float limit = limit_of(bound);
         auto queue_groups = [&] {
             for (int i = 0; i < steps; ++i)
-                if (Elem<T>::get(sh.group_max[i][tid]) > limit) sh.queue[atomicAdd(&sh.queued, 1)] = (uint16_t)(i * NT + tid);
+                if (Elem<T>::get(group_max[i][tid]) > limit) queue[atomicAdd(&sh.queued, 1)] = (uint16_t)(i * NT + tid);
             row_sync<NW>();
             return sh.queued;
         };
@@ -533,7 +549,7 @@ template <typename T, int NW> __global__ void __launch_bounds__(NW == 1 ? 128 : 
                 int at[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int g = sh.queue[min(q + j * NW, n - 1)];
+                    const int g = queue[min(q + j * NW, n - 1)];
                     const int v = begin + (g / NT) * NT * U + (lane / E) * NT + g % NT;
                     at[j] = v * E + lane % E;
                     const bool in = q + j * NW < n && lane < U * E && v < stop && at[j] >= r.head && at[j] < r.end;
@@ -631,14 +647,19 @@ template <typename T> int launch_logprobs(tb_ctx* ctx, LogprobArgs p) {
     constexpr int E = 16 / sizeof(T);
     const int64_t chunks = ceil_div(p.vocab, E) + 1;  // one more where a row starts inside a chunk
     const int64_t step = 32 * LP_U;                   // chunks a step of one warp
-    // Warps per row: the fewest (they share the work at a row's end, which the others wait for) that keep
-    // 20 warps on every SM and a part within LP_STEPS steps: @@W@@
+    // Warps per row: the fewest (a row's end keeps few of them busy) that put 20 warps on every SM and leave a part
+    // within lp_steps() steps: @@W@@
     int nw = 1;
-    while (nw < 8 && chunks > step * nw + 1 && (p.rows * nw < 20 * ctx->sm_count || chunks > step * nw * LP_STEPS<T>)) nw *= 2;
-    // with 8 a row goes in parts of a step each at least while the CTAs do not fill the GPU, and of LP_STEPS at most
-    const int64_t steps = ceil_div(chunks, step * nw);
-    p.splits = 1;
-    if (nw == 8) p.splits = (int)std::max<int64_t>(std::min<int64_t>({steps, 4 * ctx->sm_count / p.rows, 256}), ceil_div(steps, LP_STEPS<T>));
+    while (nw < 8 && chunks > step * nw + 1 && (p.rows * nw < 20 * ctx->sm_count || chunks > step * nw * lp_steps<T>(nw))) nw *= 2;
+    // With 8, a row goes in parts of a step each at least while the CTAs do not fill the GPU. From 3 steps on the next
+    // step's loads are taken under this one's sums, with 24 warps to an SM instead of 32: not where that makes a second wave.
+    const int64_t steps = ceil_div(chunks, step * nw), sms = ctx->sm_count, least = ceil_div(steps, lp_steps<T>(nw));
+    auto parts = [&](int64_t ctas) { return nw == 8 ? std::max<int64_t>(std::min<int64_t>({steps, ctas * sms / p.rows, 256}), least) : 1; };
+    p.splits = (int)parts(4);
+    const int64_t warps = p.rows * p.splits * nw;
+    const bool ahead = ceil_div(steps, p.splits) >= 3 && (p.splits > 1 || warps <= 24 * sms || warps > 32 * sms);
+    if (ahead) p.splits = (int)parts(3);
+    p.steps = (int)ceil_div(steps, p.splits);
     if (p.rows * p.splits > 2147483647) return fail(TB_ERR_UNSUPPORTED, "token logprobs: too many rows");
     if (p.splits > 1) {
         // partial results and counters (the context's own, always left at 0, are too few for many long rows)
@@ -653,12 +674,17 @@ template <typename T> int launch_logprobs(tb_ctx* ctx, LogprobArgs p) {
             TB_CHECK_CUDA(cudaMemsetAsync(p.counters, 0, p.rows * sizeof(int), ctx->stream));
         }
     }
+    const size_t smem = p.top ? (size_t)(nw == 1 ? 4 : nw) * 32 * p.steps * (sizeof(T) + 2) : 0;
     const dim3 grid((unsigned)(nw == 1 ? ceil_div(p.rows, 4) : p.rows * p.splits)), block((unsigned)(nw == 1 ? 128 : nw * 32));
+    auto run = [&](auto n, auto a) {
+        return launch_early(ctx, "k_token_logprobs", k_token_logprobs<T, decltype(n)::value, decltype(a)::value>, grid, block, smem, p);
+    };
+    auto pick = [&](auto n) { return ahead ? run(n, std::true_type()) : run(n, std::false_type()); };
     switch (nw) {
-    case 1: return launch_early(ctx, "k_token_logprobs", k_token_logprobs<T, 1>, grid, block, 0, p);
-    case 2: return launch_early(ctx, "k_token_logprobs", k_token_logprobs<T, 2>, grid, block, 0, p);
-    case 4: return launch_early(ctx, "k_token_logprobs", k_token_logprobs<T, 4>, grid, block, 0, p);
-    default: return launch_early(ctx, "k_token_logprobs", k_token_logprobs<T, 8>, grid, block, 0, p);
+    case 1: return pick(std::integral_constant<int, 1>());
+    case 2: return pick(std::integral_constant<int, 2>());
+    case 4: return pick(std::integral_constant<int, 4>());
+    default: return pick(std::integral_constant<int, 8>());
     }
 }
 
@@ -783,7 +809,7 @@ int tb_token_logprobs_fwd(tb_ctx* ctx, int64_t rows, int64_t vocab, const void* 
     if (top > TOP_MAX) return fail(TB_ERR_UNSUPPORTED, "token logprobs: top over %d", TOP_MAX);
     if (rows == 0) return TB_OK;
     if ((tokens && !logprob) || (top && (!top_logprob || !top_token))) return fail(TB_ERR_INVALID, "token logprobs: null pointer");
-    LogprobArgs p{rows, vocab, logits, stride, tokens, 1.f / temperature, (int)top, tokens ? logprob : nullptr, entropy, lse, row_max, log_sum, top_logprob, top_token, 1, nullptr, nullptr};
+    LogprobArgs p{rows, vocab, logits, stride, tokens, 1.f / temperature, (int)top, tokens ? logprob : nullptr, entropy, lse, row_max, log_sum, top_logprob, top_token, 0, 1, nullptr, nullptr};
     return elem_dispatch(type, [&](auto t) { return launch_logprobs<decltype(t)>(ctx, p); });
 }
 
