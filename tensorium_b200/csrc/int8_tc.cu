@@ -8,10 +8,9 @@
 // 128-byte swizzled rows; TMA fills zeros past k, m and n, so no size needs padding. int32 sums are
 // exact in any order, which is what lets k be split freely.
 //
-// k_int8_stream: one CTA per SM on tiles of 128 channels x up to 128 tokens. Tiles that do not fill a wave of SMs are
-// shared out by k, to the byte evenly, since one SM streams from HBM at 43 GB/s at most (measured, with 5 as
-// with 10 stages in flight): only with equal shares do all of them together reach its rate. The CTAs of a tile leave
-// int32 sums in the workspace, and the last of them to finish adds them.
+// k_int8_stream: one CTA per SM on tiles of 128 channels x up to 128 tokens. One SM streams from HBM at 43 to 48 GB/s at
+// most (measured, with 5 as with 10 stages in flight), so a few long tiles are shared out by k, to
+// 128 bytes evenly: the CTAs of a tile leave int32 sums in the workspace, and the last of them to finish adds them.
 // k_int8_pair: persistent CTA pairs (cta_group::2) on 256 x 256 tiles with two accumulators in
 // TMEM, so the epilogue of one tile runs under the products of the next.
 //
@@ -520,32 +519,38 @@ int launch_cluster(tb_ctx* ctx, const char* what, dim3 grid, int threads, int sm
     return check_launch(what);
 }
 
+// Tokens of a shared tile: up to 128, in as many equal tiles as it takes.
+int stream_tokens(int64_t m) { return (int)round_up(ceil_div(m, ceil_div(m, 128)), 16); }
+
 // `scratch`: where the workspace is free
-int launch_stream(tb_ctx* ctx, const Int8Args& p, int64_t y_type, bool early, int bt, size_t scratch) {
+int launch_stream(tb_ctx* ctx, const Int8Args& p, int64_t y_type, bool early, size_t scratch) {
+    // Whole tiles, or (one wave of them at most) k shared out evenly over all SMs. In whole tiles an SM takes
+    // 0.34 us for 128 bytes of k, whatever its tokens: the weights' 16 KB at 48 bytes a nanosecond. So the tokens go in as
+    // many tiles as one wave holds, which shortens the epilogues (128 x 4096 x 4096: 14.3 us on tiles of 32
+    // tokens, 15.0 of 128). Sharing adds 6 us and 0.04 for each token of a tile, to leave and add the partial sums (32 x 4096 x
+    // 16384: 21 us shared, 48 whole; 128 x 4096 x 4096: 18 shared).
+    const int64_t sms = ctx->sm_count, ktiles = ceil_div(p.k, I8_BK), tiles_n = ceil_div(p.n, 128), least = ceil_div(p.m, 128);
+    const int64_t most = std::max(least, std::min(ceil_div(p.m, 16), sms / tiles_n));
+    int bt = (int)round_up(ceil_div(p.m, most), 16);
+    const int sk_bt = stream_tokens(p.m);
+    const int64_t sk_tiles = least * tiles_n, sk_grid = std::min(sms, ceil_div(sk_tiles * ktiles, 4));
+    const double whole = 0.34 * (double)(ktiles * ceil_div(ceil_div(p.m, bt) * tiles_n, sms));
+    const double shared = 0.34 * (double)(sk_tiles * ktiles) / (double)sk_grid + 6 + 0.04 * sk_bt;
+    const bool share = sk_tiles < sms && sk_grid > sk_tiles && shared < whole;
+    if (share) bt = sk_bt;
     I8Maps maps;
     int r = encode_rows(&maps.w, p.w, p.k, p.n, p.w_stride, 128);
     if (r == TB_OK) r = encode_rows(&maps.a, p.a, p.k, p.m, p.a_stride, bt);
     if (r != TB_OK) return r;
-    const int64_t tiles_m = ceil_div(p.m, bt), tiles = tiles_m * ceil_div(p.n, 128), ktiles = ceil_div(p.k, I8_BK), sms = ctx->sm_count;
+    const int64_t tiles_m = ceil_div(p.m, bt), tiles = tiles_m * tiles_n;
     StreamArgs g = {};
     g.bt = bt;
     g.stages = (int)std::min<int64_t>(I8S_MAX_STAGES, (I8S_SMEM - 1024) / (I8_W_BYTES + bt * I8_BK));
     g.tiles_m = (int)tiles_m;
     g.ktiles = (int)ktiles;
-    // Whole tiles in full waves; what is left of one wave, with the wave before it, is shared out evenly (in
-    // pieces of 4 units at least on average) where that saves more than leaving and adding the partial sums costs: 4 us, in
-    // which an SM loads 40 bytes a nanosecond.
-    int64_t grid = std::min(tiles, sms);
-    if (tiles % sms != 0) {
-        const int64_t sk = tiles < sms ? tiles : tiles % sms + sms, unit = I8_W_BYTES + bt * I8_BK;
-        const int64_t sk_grid = std::min(sms, ceil_div(sk * ktiles, 4));
-        const double whole = (double)ceil_div(sk, sms) * ktiles * unit / 40, shared = (double)sk * ktiles * unit / sk_grid / 40 + 4000;
-        if (sk_grid > std::min(tiles, sms) - (tiles > sms) && shared < whole) {
-            g.sk_tiles = (int)sk;
-            grid = sk_grid;
-        }
-    }
+    g.sk_tiles = share ? (int)tiles : 0;
     g.dp_tiles = (int)(tiles - g.sk_tiles);
+    const int64_t grid = share ? sk_grid : std::min(tiles, sms);
     if (g.sk_tiles) {
         const size_t need = scratch + (size_t)grid * 2 * bt * 128 * 4;
         if (need > ctx->ws_bytes && scratch) return fail(TB_ERR_STATE, "int8 product: workspace not reserved");
@@ -575,9 +580,6 @@ int launch_pair(tb_ctx* ctx, const Int8Args& p, int64_t y_type, bool early) {
 
 }  // namespace
 
-// Tokens of a tile of the single-CTA kernel: up to 128 in as many equal tiles as it takes.
-static int stream_tokens(int64_t m) { return (int)round_up(ceil_div(m, ceil_div(m, 128)), 16); }
-
 size_t int8_gemm_scratch(const tb_ctx* ctx, int64_t m) { return (size_t)ctx->sm_count * 2 * stream_tokens(m) * 128 * 4; }
 
 int int8_gemm_tc(tb_ctx* ctx, const Int8Args& p, int64_t y_type, bool early, size_t scratch) {
@@ -586,7 +588,7 @@ int int8_gemm_tc(tb_ctx* ctx, const Int8Args& p, int64_t y_type, bool early, siz
     const int64_t tiles = ceil_div(p.m, 128) * ceil_div(p.n, 128);
     if ((p.m > 128 && ceil_div(p.m, 256) * ceil_div(p.n, 256) * 2 * 3 >= sms * 2) || tiles * ceil_div(p.k, I8_BK) >= ((int64_t)1 << 30))
         return launch_pair(ctx, p, y_type, early);
-    return launch_stream(ctx, p, y_type, early, stream_tokens(p.m), scratch);
+    return launch_stream(ctx, p, y_type, early, scratch);
 }
 
 }  // namespace tbi
