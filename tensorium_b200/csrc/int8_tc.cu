@@ -520,39 +520,52 @@ int launch_cluster(tb_ctx* ctx, const char* what, dim3 grid, int threads, int sm
 }
 
 // Tokens of a shared tile: up to 128, in as many equal tiles as it takes.
-int stream_tokens(int64_t m) { return (int)round_up(ceil_div(m, ceil_div(m, 128)), 16); }
+int shared_tokens(int64_t m) { return (int)round_up(ceil_div(m, ceil_div(m, 128)), 16); }
+
+// How a product is run: the fastest of three by what they were measured to take, us, for `ktiles` steps of 128 bytes
+// of k. Whole tiles of one CTA, 4.5 + 0.34 a step and wave: an SM takes that for a step whatever its tokens, the weights' 16 KB at
+// 48 bytes a nanosecond; so the tokens go in as many tiles as one wave holds, which shortens the epilogues (128 x
+// 4096 x 4096: 14.3 on tiles of 32 tokens, 15.0 of 128). One wave of tiles at most, shared out by k evenly over all SMs: 6 and
+// 0.04 a token of the tile more, to leave and add the partial sums (32 x 4096 x 16384: 21 shared, 48 whole; 128 x
+// 4096 x 4096: 18 shared). Tiles of CTA pairs, 7.5 + 0.36 a step and wave for four times the work (1000 x 4096 x
+// 4096: 19, and 26 in whole tiles; 512 x 4096 x 4096: 19 and 16).
+struct Plan {
+    int bt;        // tokens of a tile of the single-CTA kernel, 0 for pairs
+    bool share;
+    int64_t grid;
+};
+
+Plan plan(const tb_ctx* ctx, int64_t m, int64_t n, int64_t k) {
+    const int64_t sms = ctx->sm_count, ktiles = ceil_div(k, I8_BK), tiles_n = ceil_div(n, 128), least = ceil_div(m, 128);
+    const int64_t most = std::max(least, std::min(ceil_div(m, 16), sms / tiles_n));
+    const int bt = (int)round_up(ceil_div(m, most), 16), sk_bt = shared_tokens(m);
+    const int64_t tiles = ceil_div(m, bt) * tiles_n, sk_tiles = least * tiles_n, sk_grid = std::min(sms, ceil_div(sk_tiles * ktiles, 4));
+    const double whole = 4.5 + 0.34 * (double)(ktiles * ceil_div(tiles, sms));
+    const bool can_share = sk_tiles < sms && sk_grid > sk_tiles;
+    const double shared = can_share ? 10.5 + 0.04 * sk_bt + 0.34 * (double)(sk_tiles * ktiles) / (double)sk_grid : 1e30;
+    const double pair = m > 128 ? 7.5 + 0.36 * (double)(ktiles * ceil_div(ceil_div(m, 256) * ceil_div(n, 256), sms / 2)) : 1e30;
+    if (pair < whole && pair < shared) return {0, false, 0};
+    if (tiles * ktiles >= ((int64_t)1 << 30)) return {0, false, 0};  // the single-CTA kernel counts in 32 bits
+    return shared < whole ? Plan{sk_bt, true, sk_grid} : Plan{bt, false, std::min(tiles, sms)};
+}
 
 // `scratch`: where the workspace is free
-int launch_stream(tb_ctx* ctx, const Int8Args& p, int64_t y_type, bool early, size_t scratch) {
-    // Whole tiles, or (one wave of them at most) k shared out evenly over all SMs. In whole tiles an SM takes
-    // 0.34 us for 128 bytes of k, whatever its tokens: the weights' 16 KB at 48 bytes a nanosecond. So the tokens go in as
-    // many tiles as one wave holds, which shortens the epilogues (128 x 4096 x 4096: 14.3 us on tiles of 32
-    // tokens, 15.0 of 128). Sharing adds 6 us and 0.04 for each token of a tile, to leave and add the partial sums (32 x 4096 x
-    // 16384: 21 us shared, 48 whole; 128 x 4096 x 4096: 18 shared).
-    const int64_t sms = ctx->sm_count, ktiles = ceil_div(p.k, I8_BK), tiles_n = ceil_div(p.n, 128), least = ceil_div(p.m, 128);
-    const int64_t most = std::max(least, std::min(ceil_div(p.m, 16), sms / tiles_n));
-    int bt = (int)round_up(ceil_div(p.m, most), 16);
-    const int sk_bt = stream_tokens(p.m);
-    const int64_t sk_tiles = least * tiles_n, sk_grid = std::min(sms, ceil_div(sk_tiles * ktiles, 4));
-    const double whole = 0.34 * (double)(ktiles * ceil_div(ceil_div(p.m, bt) * tiles_n, sms));
-    const double shared = 0.34 * (double)(sk_tiles * ktiles) / (double)sk_grid + 6 + 0.04 * sk_bt;
-    const bool share = sk_tiles < sms && sk_grid > sk_tiles && shared < whole;
-    if (share) bt = sk_bt;
+int launch_stream(tb_ctx* ctx, const Int8Args& p, int64_t y_type, bool early, const Plan& plan, size_t scratch) {
+    const int bt = plan.bt;
+    const int64_t tiles_m = ceil_div(p.m, bt), tiles = tiles_m * ceil_div(p.n, 128);
     I8Maps maps;
     int r = encode_rows(&maps.w, p.w, p.k, p.n, p.w_stride, 128);
     if (r == TB_OK) r = encode_rows(&maps.a, p.a, p.k, p.m, p.a_stride, bt);
     if (r != TB_OK) return r;
-    const int64_t tiles_m = ceil_div(p.m, bt), tiles = tiles_m * tiles_n;
     StreamArgs g = {};
     g.bt = bt;
     g.stages = (int)std::min<int64_t>(I8S_MAX_STAGES, (I8S_SMEM - 1024) / (I8_W_BYTES + bt * I8_BK));
     g.tiles_m = (int)tiles_m;
-    g.ktiles = (int)ktiles;
-    g.sk_tiles = share ? (int)tiles : 0;
+    g.ktiles = (int)ceil_div(p.k, I8_BK);
+    g.sk_tiles = plan.share ? (int)tiles : 0;
     g.dp_tiles = (int)(tiles - g.sk_tiles);
-    const int64_t grid = share ? sk_grid : std::min(tiles, sms);
     if (g.sk_tiles) {
-        const size_t need = scratch + (size_t)grid * 2 * bt * 128 * 4;
+        const size_t need = scratch + (size_t)plan.grid * 2 * bt * 128 * 4;
         if (need > ctx->ws_bytes && scratch) return fail(TB_ERR_STATE, "int8 product: workspace not reserved");
         if ((r = ensure_workspace(ctx, need)) != TB_OK) return r;
         g.partial = reinterpret_cast<int*>(static_cast<char*>(ctx->ws) + scratch);
@@ -560,7 +573,7 @@ int launch_stream(tb_ctx* ctx, const Int8Args& p, int64_t y_type, bool early, si
     }
     const int smem = g.stages * (I8_W_BYTES + bt * I8_BK) + 1024;
     return elem_dispatch(y_type, [&](auto t) {
-        return launch_cluster<k_int8_stream<decltype(t)>>(ctx, "k_int8_stream", dim3((unsigned)grid), I8S_THREADS, smem, I8S_SMEM, dim3(1, 1, 1),
+        return launch_cluster<k_int8_stream<decltype(t)>>(ctx, "k_int8_stream", dim3((unsigned)plan.grid), I8S_THREADS, smem, I8S_SMEM, dim3(1, 1, 1),
                                                           early, maps, p, g, ctx->d_status);
     });
 }
@@ -580,15 +593,11 @@ int launch_pair(tb_ctx* ctx, const Int8Args& p, int64_t y_type, bool early) {
 
 }  // namespace
 
-size_t int8_gemm_scratch(const tb_ctx* ctx, int64_t m) { return (size_t)ctx->sm_count * 2 * stream_tokens(m) * 128 * 4; }
+size_t int8_gemm_scratch(const tb_ctx* ctx, int64_t m) { return (size_t)ctx->sm_count * 2 * shared_tokens(m) * 128 * 4; }
 
 int int8_gemm_tc(tb_ctx* ctx, const Int8Args& p, int64_t y_type, bool early, size_t scratch) {
-    const int64_t sms = ctx->sm_count;
-    // pairs once their tiles occupy two thirds of the SMs
-    const int64_t tiles = ceil_div(p.m, 128) * ceil_div(p.n, 128);
-    if ((p.m > 128 && ceil_div(p.m, 256) * ceil_div(p.n, 256) * 2 * 3 >= sms * 2) || tiles * ceil_div(p.k, I8_BK) >= ((int64_t)1 << 30))
-        return launch_pair(ctx, p, y_type, early);
-    return launch_stream(ctx, p, y_type, early, scratch);
+    const Plan pl = plan(ctx, p.m, p.n, p.k);
+    return pl.bt ? launch_stream(ctx, p, y_type, early, pl, scratch) : launch_pair(ctx, p, y_type, early);
 }
 
 }  // namespace tbi
