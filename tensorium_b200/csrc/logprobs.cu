@@ -100,6 +100,7 @@ constexpr float EXP_FLOOR = -200.f;
 template <typename T> struct Chunk;
 template <> struct Chunk<float> {
     static constexpr uint32_t MASKED = 0xff800000u;  // -infinity
+    static constexpr float LOWEST = -0x1.fffffep127f;  // the type's lowest finite value
     // the largest logit of n chunks, NaN if one is
     template <int N> static __device__ __forceinline__ float vmax(const uint4 (&r)[N]) {
         float m = -INFINITY;
@@ -123,6 +124,7 @@ template <> struct Chunk<float> {
 };
 template <> struct Chunk<__nv_bfloat16> {
     static constexpr uint32_t MASKED = 0xff80ff80u;
+    static constexpr float LOWEST = -0x1.fep127f;
     template <int N> static __device__ __forceinline__ float vmax(const uint4 (&r)[N]) {
         auto h = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
         __nv_bfloat162 m[N];
@@ -148,6 +150,7 @@ template <> struct Chunk<__nv_bfloat16> {
 };
 template <> struct Chunk<__half> {
     static constexpr uint32_t MASKED = 0xfc00fc00u;
+    static constexpr float LOWEST = -65504.f;
     template <int N> static __device__ __forceinline__ float vmax(const uint4 (&r)[N]) {
         auto h = [](uint32_t w) { return *reinterpret_cast<const __half2*>(&w); };
         __half2 m[N];
@@ -328,22 +331,35 @@ struct Given {
     }
 };
 
-// Results of one row, by one warp that holds its sums and its best keys.
-__device__ __forceinline__ void write_row(const LogprobArgs& p, int64_t row, const Sums& a, unsigned long long list, const Given& given, int lane) {
-    const bool empty = a.max == -INFINITY;
-    const float logz = logf(a.z);
-    auto logprob = [&](float v) {
-        return a.bad ? nan_f() : empty ? -INFINITY : __fsub_rn(__fmul_rn(__fsub_rn(v, a.max), p.inv_t), logz);
-    };
-    if (lane == 0) {
+// A row's results from its sums.
+struct RowLog {
+    Sums a;
+    bool empty;
+    float inv_t, logz;
+    __device__ __forceinline__ RowLog(const LogprobArgs& p, const Sums& s) : a(s), empty(s.max == -INFINITY), inv_t(p.inv_t), logz(logf(s.z)) {}
+    __device__ __forceinline__ float of(float v) const {
+        return a.bad ? nan_f() : empty ? -INFINITY : __fsub_rn(__fmul_rn(__fsub_rn(v, a.max), inv_t), logz);
+    }
+    // by one thread
+    __device__ __forceinline__ void write(const LogprobArgs& p, int64_t row, const Given& given) const {
         if (p.logprob)
-            p.logprob[row] = given.token >= p.vocab ? nan_f() : given.token < 0 ? (a.bad ? nan_f() : 0.f) : logprob(given.logit);
+            p.logprob[row] = given.token >= p.vocab ? nan_f() : given.token < 0 ? (a.bad ? nan_f() : 0.f) : of(given.logit);
         if (p.entropy)
             p.entropy[row] = a.bad ? nan_f() : empty ? 0.f : fmaxf(__fsub_rn(logz, __fmul_rn(__fdiv_rn(a.s, a.z), LN2)), 0.f);
-        if (p.lse) p.lse[row] = a.bad ? nan_f() : empty ? -INFINITY : __fadd_rn(__fmul_rn(a.max, p.inv_t), logz);
+        if (p.lse) p.lse[row] = a.bad ? nan_f() : empty ? -INFINITY : __fadd_rn(__fmul_rn(a.max, inv_t), logz);
         if (p.row_max) p.row_max[row] = a.bad ? nan_f() : a.max;
         if (p.log_sum) p.log_sum[row] = a.bad ? nan_f() : empty ? 0.f : logz;
     }
+    __device__ __forceinline__ void write_top(const LogprobArgs& p, int64_t row, int i, unsigned long long key) const {
+        p.top_token[row * p.top + i] = a.bad ? -1 : (int64_t)key_col(key);
+        p.top_logprob[row * p.top + i] = of(key_val(key));
+    }
+};
+
+// Results of one row, by one warp that holds its sums and its best keys.
+__device__ __forceinline__ void write_row(const LogprobArgs& p, int64_t row, const Sums& a, unsigned long long list, const Given& given, int lane) {
+    const RowLog log(p, a);
+    if (lane == 0) log.write(p, row, given);
     if (p.top == 0) return;
     const int have = min(__popc(__ballot_sync(0xffffffffu, list != 0)), p.top);
     if (have < p.top) {
@@ -359,10 +375,7 @@ __device__ __forceinline__ void write_row(const LogprobArgs& p, int64_t row, con
         for (int i = have; i < lane; ++i) left &= left - 1;  // the (lane - have)-th of them
         if (lane >= have) list = top_key(-INFINITY, (uint32_t)(__ffsll((long long)left) - 1));
     }
-    if (lane < p.top) {
-        p.top_token[row * p.top + lane] = a.bad ? -1 : (int64_t)key_col(list);
-        p.top_logprob[row * p.top + lane] = logprob(key_val(list));
-    }
+    if (lane < p.top) log.write_top(p, row, lane, list);
 }
 
 // The sums of one thread: against a reference of its own, an earlier logit, moved only when a logit is
@@ -450,8 +463,9 @@ __device__ __forceinline__ void take(unsigned long long& list, unsigned long lon
 // pass only the groups that can hold one of the best are read again: those whose maximum reaches the k-th
 // largest of the threads' maxima, about k of them.
 constexpr int LP_U = 4;
-// most steps of a part: 32 KB of groups to a CTA, and what an SM's threads share (float: 45 and 30)
-template <typename T> int lp_steps(int nw) { return nw == 8 ? (sizeof(T) == 4 ? 28 : 32) : (sizeof(T) == 4 ? 40 : 64); }
+// Most steps of a part: a CTA's groups fit its shared memory, and longer rows are faster on more warps (4096 x 131072 bf16 top
+// 20: 198 us on 4, 222 on 2).
+template <typename T> int lp_steps(int nw) { return nw < 8 ? 40 : sizeof(T) == 4 ? 28 : 32; }
 
 constexpr int KEYS = 64;  // candidates that are ranked against one another
 
@@ -643,14 +657,157 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? (AHEAD ? 6 
     if (warp == 0) write_row(p, row, w, list, given, lane);
 }
 
+// ---- forward, short rows ----------------------------------------------------------------------------
+// L lanes to a row of up to SHORT_U chunks a lane and up to SHORT_TOP alternatives, all of it in registers: 32 / L rows share a
+// warp's instructions for what comes after the logits (joining the sums, ranking, logarithms), which are most of
+// a short row's work.
+constexpr int SHORT_U = 8, SHORT_TOP = 8, SHORT_KEYS = 32;
+
+template <int L, typename V, typename F> __device__ __forceinline__ V group_reduce(V v, F f) {
+#pragma unroll
+    for (int o = L / 2; o; o /= 2) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+template <typename T, int L> __global__ void __launch_bounds__(128, 6) k_token_logprobs_short(const LogprobArgs p) {
+    TB_GRID_DEP_ENTRY();
+    constexpr int E = 16 / sizeof(T), U = SHORT_U, G = 32 / L;
+    __shared__ unsigned long long found[4][G][SHORT_KEYS];
+    __shared__ int nfound[4][G];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gl = lane % L, group = lane / L;
+    const int64_t mine = ((int64_t)blockIdx.x * 4 + warp) * G + group, row = min(mine, p.rows - 1);  // every lane stays for the shuffles
+    const bool active = mine < p.rows;
+    const T* x = static_cast<const T*>(p.logits) + row * p.stride;
+    const Row<T> r(x, p.vocab);
+    const int stop = r.chunks();
+    const float c = __fmul_rn(LOG2E, p.inv_t);
+
+    uint4 raw[U];
+    if (__all_sync(0xffffffffu, r.head == 0 && r.end % E == 0)) {
+        const uint4* q = reinterpret_cast<const uint4*>(r.base) + gl;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            raw[u] = make_uint4(Chunk<T>::MASKED, Chunk<T>::MASKED, Chunk<T>::MASKED, Chunk<T>::MASKED);
+            if (u * L + gl < stop) raw[u] = q[u * L];
+        }
+    } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u) raw[u] = r.load(u * L + gl, stop);
+    }
+    Given given;
+    if (gl == 0) given.read(p, row, x);
+    if (gl == 0) nfound[warp][group] = 0;
+
+    const float own = Chunk<T>::vmax(raw);  // NaN if one of the lane's is
+    Running a;
+    a.max = group_reduce<L>(own, max_nan);
+    a.bad = !(a.max < INFINITY);
+    a.ref = a.bad ? 0.f : a.max;
+    bool clamp = __any_sync(0xffffffffu, a.max == -INFINITY);
+#pragma unroll
+    for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (u * L + gl >= stop) continue;
+            if (clamp) a.add<T, true>(raw[u], c);
+            else a.add<T, false>(raw[u], c);
+        }
+        if (clamp) break;
+        const float t = __fadd_rn(a.s.x, a.s.y);
+        clamp = __any_sync(0xffffffffu, t != t);  // masked logits: again, with the clamp
+        if (!clamp) break;
+        a.z = a.s = {0.f, 0.f};
+    }
+    const auto add = [](float v, float w) { return __fadd_rn(v, w); };
+    const Sums w = {a.max, group_reduce<L>(__fadd_rn(a.z.x, a.z.y), add), group_reduce<L>(__fadd_rn(a.s.x, a.s.y), add), a.bad};
+    const RowLog log(p, w);
+    if (gl == 0 && active) log.write(p, row, given);
+    if (p.top == 0) return;
+
+    // the k-th largest of the lanes' maxima bounds the k-th best from below
+    uint32_t best = ordered(own), bound = 0;
+    for (int i = 0; i < p.top; ++i) {
+        bound = group_reduce<L>(best, [](uint32_t v, uint32_t w) { return max(v, w); });
+        if (best == bound) best = 0;
+    }
+    const float least = bound > ordered(-INFINITY) && !a.bad ? unordered(bound) : Chunk<T>::LOWEST;
+    uint32_t some[2] = {0, 0};  // bit u * E + e
+#pragma unroll
+    for (int u = 0; u < U; ++u) some[u * E / 32] |= Chunk<T>::at_least(raw[u], least) << u * E % 32;
+    const int n = group_reduce<L>(__popc(some[0]) + __popc(some[1]), [](int v, int w) { return v + w; });
+    unsigned long long* keys = found[warp][group];
+    __syncwarp();
+    if (n <= SHORT_KEYS) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            while (some[h]) {
+                const int i = __ffs((int)some[h]) - 1 + 32 * h;
+                some[h] &= some[h] - 1;
+                const int at = (i / E * L + gl) * E + i % E;
+                keys[atomicAdd(&nfound[warp][group], 1)] = top_key(Elem<T>::get(r.base[at]), (uint32_t)(at - r.head));
+            }
+    }
+    __syncwarp();
+    if (n <= SHORT_KEYS) {
+        for (int i = gl; i < n; i += L) {
+            const unsigned long long k = keys[i];
+            int rank = 0;
+            for (int j = 0; j < n; ++j) rank += keys[j] > k;
+            if (rank < p.top && active) log.write_top(p, row, rank, k);
+        }
+        if (n < p.top && gl == 0 && active) {  // fewer columns than alternatives are not masked: the lowest masked ones follow
+            uint32_t col = 0;
+            for (int i = n; i < p.top; ++i, ++col) {
+                for (int j = 0; j < n; ++j)
+                    if (key_col(keys[j]) == col) ++col, j = -1;
+                log.write_top(p, row, i, top_key(-INFINITY, col));
+            }
+        }
+    }
+    // many equal logits: the next best by another pass, for all the warp's rows or none
+    const bool many = n > SHORT_KEYS;
+    if (__any_sync(0xffffffffu, many)) {
+        unsigned long long last = ~0ull;
+        for (int i = 0; i < p.top; ++i) {
+            unsigned long long k = 0;
+            if (many)
+                for (int64_t j = gl; j < p.vocab; j += L) {
+                    const unsigned long long t = top_key(Elem<T>::get(x[j]), (uint32_t)j);
+                    if (t < last && t > k) k = t;
+                }
+            last = group_reduce<L>(k, [](unsigned long long v, unsigned long long w) { return v > w ? v : w; });
+            if (many && gl == 0 && active) log.write_top(p, row, i, last);
+        }
+    }
+}
+
 template <typename T> int launch_logprobs(tb_ctx* ctx, LogprobArgs p) {
     constexpr int E = 16 / sizeof(T);
-    const int64_t chunks = ceil_div(p.vocab, E) + 1;  // one more where a row starts inside a chunk
+    // 16-byte chunks that a row touches at most
+    const bool aligned = aligned16(p.logits) && (p.rows == 1 || p.stride % E == 0);
+    const int64_t chunks = ceil_div(p.vocab + (aligned ? 0 : E - 1), E);
     const int64_t step = 32 * LP_U;                   // chunks a step of one warp
     // Warps per row: the fewest (a row's end keeps few of them busy) that put 20 warps on every SM and leave a part
-    // within lp_steps() steps: @@W@@
+    // within lp_steps() steps. Measured with 1 / 2 / 4 / 8 warps, us: 8192 x 2048 bf16 top 5 18.7 / 25.7 / 47 / 88, 4096 x 32000 60 / 63 / 65 /
+    // 77, 1000 x 16000 22.8 / 16.3 / 13.7 / 17.6, 777 x 30001 f32 46 / 27.8 / 19.9 / 23.0.
+    // Short rows share warps where they fill the GPU that way, or need no alternatives (else a warp to a row has the shorter
+    // chain, and finds more of them): 16384 x 1000 f16 top 5 in 15.9 us and 21.0 with a warp each, 16384 x 80 8.7 and
+    // 17.7, 60000 x 10 24.7 and 65.6; 200 x 200 4.7 and 4.0.
+    const int lanes = chunks <= 4 * SHORT_U && p.top <= 4 ? 4 : chunks <= 8 * SHORT_U ? 8 : chunks <= 16 * SHORT_U ? 16 : 32;
+    if (chunks <= lanes * SHORT_U && p.top <= SHORT_TOP && (p.top == 0 || p.rows * lanes / 32 >= 8 * ctx->sm_count)) {
+        auto run = [&](auto n) {
+            return launch_early(ctx, "k_token_logprobs_short", k_token_logprobs_short<T, decltype(n)::value>, dim3((unsigned)ceil_div(p.rows, 128 / lanes)),
+                                dim3(128), 0, p);
+        };
+        switch (lanes) {
+        case 4: return run(std::integral_constant<int, 4>());
+        case 8: return run(std::integral_constant<int, 8>());
+        case 16: return run(std::integral_constant<int, 16>());
+        default: return run(std::integral_constant<int, 32>());
+        }
+    }
     int nw = 1;
-    while (nw < 8 && chunks > step * nw + 1 && (p.rows * nw < 20 * ctx->sm_count || chunks > step * nw * lp_steps<T>(nw))) nw *= 2;
+    while (nw < 8 && chunks > step * nw && (p.rows * nw < 20 * ctx->sm_count || chunks > step * nw * lp_steps<T>(nw))) nw *= 2;
     // With 8, a row goes in parts of a step each at least while the CTAs do not fill the GPU. From 3 steps on the next
     // step's loads are taken under this one's sums, with 24 warps to an SM instead of 32: not where that makes a second wave.
     const int64_t steps = ceil_div(chunks, step * nw), sms = ctx->sm_count, least = ceil_div(steps, lp_steps<T>(nw));
@@ -773,7 +930,8 @@ template <typename T, bool WARP> __global__ void __launch_bounds__(256) k_token_
 
 template <typename T> int launch_bwd(tb_ctx* ctx, LogprobBwdArgs p) {
     constexpr int E = 16 / sizeof(T);
-    const int64_t chunks = ceil_div(p.vocab, E) + 1;  // one more where a row starts inside a chunk
+    const bool aligned = aligned16(p.logits) && (p.rows == 1 || p.stride % E == 0);
+    const int64_t chunks = ceil_div(p.vocab + (aligned ? 0 : E - 1), E);
     if (chunks <= 32 * 4)
         return launch_early(ctx, "k_token_logprobs_bwd", k_token_logprobs_bwd<T, true>, dim3((unsigned)ceil_div(p.rows, 8)), dim3(256), 0, p);
     p.parts = ceil_div(chunks, 256 * 4);

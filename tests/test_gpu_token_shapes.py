@@ -49,6 +49,49 @@ def test_logprobs(ctx, rows, vocab, dtype):
     assert torch.all(torch.isfinite(r.entropy)) and torch.all(r.entropy >= 0)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("vocab", [1, 3, 10, 33, 80, 128, 129, 255, 500, 511, 1000, 1003, 1024, 2040, 2048])
+def test_short_rows(ctx, vocab, dtype):
+    """Many rows that share warps: beside ordinary ones, rows of equal and of few different logits, masked but for a
+    few columns or for none, with NaN and infinities, tokens not given or out of range."""
+    rows = 10007
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    wide = torch.full((rows, vocab + 3), torch.nan, device="cuda", dtype=TYPES[dtype])
+    logits = (3 * torch.randn(rows, vocab, device="cuda", generator=g)).to(TYPES[dtype])
+    tokens = torch.randint(vocab, (rows,), device="cuda", generator=g)
+    special = torch.arange(100, 112, device="cuda")
+    logits[100] = 1.25
+    logits[101] = -torch.inf
+    logits[102] = -torch.inf
+    logits[102, vocab // 2] = 4
+    logits[103, vocab // 3] = torch.nan
+    logits[104, vocab - 1] = torch.inf
+    logits[105] = torch.finfo(TYPES[dtype]).min
+    logits[106] = torch.where(torch.arange(vocab, device="cuda") % 3 == 1, 0.0, -0.0).to(TYPES[dtype])
+    logits[107] = (torch.arange(vocab, device="cuda") // 9 % 4).to(TYPES[dtype])
+    logits[108, ::2] = -torch.inf
+    logits[109] = -torch.inf
+    logits[109, -2:] = 0.5
+    tokens[110], tokens[111] = -7, vocab
+    logits[-1] = 2
+    picks = sorted({*special.tolist(), 0, 1, rows - 2, rows - 1, *np.random.default_rng(1).integers(0, rows, 30).tolist()})
+    wide[:, 1:vocab + 1] = logits
+    e = R.logprobs(f64(logits[picks]), tokens[picks].cpu().numpy(), 1.1, min(8, vocab))
+    for view in (logits, wide[:, 1:vocab + 1]):
+        for top in sorted({0, 1, min(4, vocab), min(5, vocab), min(8, vocab)}):
+            r = K.token_logprobs(ctx, view, tokens, top=top, temperature=1.1)
+            pairs = [("logprobs", R.logprob_off(e["logprobs"], e["lse"], vocab)), ("entropy", R.entropy_off(e["entropy"], vocab)),
+                     ("lse", R.logprob_off(e["lse"], e["lse"], vocab))]
+            if top:
+                assert np.array_equal(r.top_tokens[picks].cpu().numpy(), e["top_tokens"][:, :top]), top
+                pairs.append(("top_logprobs", R.logprob_off(e["top_logprobs"], e["lse"][:, None], vocab)[:, :top]))
+            for name, off in pairs:
+                got, ref = f64(getattr(r, name)[picks]), e[name][:, :top] if name == "top_logprobs" else e[name]
+                fin = np.isfinite(ref)
+                assert np.array_equal(got[~fin], ref[~fin], equal_nan=True), (name, top)
+                assert np.all(np.abs(got[fin] - ref[fin]) <= off[fin]), (name, top)
+
+
 @pytest.mark.parametrize("m,n,k", [(17, 4096, 4096), (20, 130, 8192), (32, 16384, 1024), (40, 18944, 300), (64, 19000, 256), (100, 25000, 129), (128, 128, 131071),
                                    (129, 9000, 700), (200, 20000, 512), (300, 5000, 1000), (500, 2000, 3000), (600, 3700, 1111), (1500, 3300, 1111), (2048, 4096, 700),
                                    (3000, 257, 65), (5000, 1025, 400), (70000, 140, 33)])
