@@ -19,8 +19,11 @@
  *     functions that say so block.
  *   - device memory is allocated only by tb_malloc, tb_init, tb_workspace_reserve and
  *     tb_net_finalize, and by the context's scratch workspace growing on demand inside
- *     tb_conv2d_fwd (split-K partials), tb_xnor_conv_fwd (packed input bits) and
- *     tb_yolo_detect (counters). Growth is refused (TB_ERR_STATE) while the stream is being
+ *     tb_conv2d_fwd (split-K partials), tb_xnor_conv_fwd (packed input bits), tb_yolo_detect
+ *     (counters), tb_int8_connected_fwd (round_up(k, 16) + 4 bytes a token, and as tb_int8_gemm),
+ *     tb_int8_gemm (partial sums: 1 KB a token and SM, 20 MB at most) and tb_token_logprobs_fwd
+ *     (parts of rows: 272 bytes each, under 1 MB for the few rows that are split, more only with
+ *     over 114688 float or 262144 16-bit columns). Growth is refused (TB_ERR_STATE) while the stream is being
  *     captured into a CUDA graph; reserve first with tb_workspace_reserve.
  */
 #ifndef TENSORIUM_B200_H
