@@ -811,15 +811,20 @@ template <typename T> int launch_logprobs(tb_ctx* ctx, LogprobArgs p) {
     }
     int nw = 1;
     while (nw < 8 && chunks > step * nw && (p.rows * nw < 20 * ctx->sm_count || chunks > step * nw * lp_steps<T>(nw))) nw *= 2;
-    // With 8, a row goes in parts of a step each at least while the CTAs do not fill the GPU. From 3 steps on the next
-    // step's loads are taken under this one's sums (777 x 50001 f32 33 -> 28 us), with 24 warps to an SM instead of 32: not where that
-    // makes a second wave (4096 x 32000 with a warp a row 60 -> 72 us).
-    const int64_t steps = ceil_div(chunks, step * nw), sms = ctx->sm_count, least = ceil_div(steps, lp_steps<T>(nw));
-    auto parts = [&](int64_t ctas) { return nw == 8 ? std::max<int64_t>(std::min<int64_t>({steps, ctas * sms / p.rows, 256}), least) : 1; };
-    p.splits = (int)parts(4);
-    const int64_t warps = p.rows * p.splits * nw;
-    const bool ahead = ceil_div(steps, p.splits) >= 3 && (p.splits > 1 || warps <= 24 * sms || warps > 32 * sms);
-    if (ahead) p.splits = (int)parts(3);
+    // With 8, few rows go in parts: of one step while all of them have an SM each, else of two steps at least and two CTAs
+    // to an SM at most (1 x 131072 bf16 top 20 7.7 us in 16 parts, 8.1 in 8; 48 x 50001 f32 top 5 10.7 in 6, 11.7 in 12). Joining them
+    // costs what up to 6 steps take (8 x 32000 bf16 top 5 6.3 whole, 7.4 in 4 parts; 5 x 60000 8.1 and 7.4).
+    const int64_t steps = ceil_div(chunks, step * nw), sms = ctx->sm_count;
+    int64_t splits = 1;
+    if (nw == 8) {
+        if (steps > 6) splits = p.rows * steps <= sms ? steps : std::min(ceil_div(steps, 2), 2 * sms / p.rows);
+        splits = std::max<int64_t>({1, std::min<int64_t>(splits, 256), ceil_div(steps, lp_steps<T>(nw))});
+    }
+    p.splits = (int)splits;
+    // From 3 steps on the next step's loads are taken under this one's sums (777 x 50001 f32 33 -> 28 us), with 24 warps to an SM
+    // instead of 32: not where that makes a second wave (4096 x 32000 with a warp a row 60 -> 72 us).
+    const int64_t warps = p.rows * splits * nw;
+    const bool ahead = ceil_div(steps, splits) >= 3 && (warps <= 24 * sms || warps > 32 * sms);
     p.steps = (int)ceil_div(steps, p.splits);
     if (p.rows * p.splits > 2147483647) return fail(TB_ERR_UNSUPPORTED, "token logprobs: too many rows");
     if (p.splits > 1) {
