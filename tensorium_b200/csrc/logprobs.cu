@@ -663,7 +663,7 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? (AHEAD ? 6 
 // ---- forward, short rows ----------------------------------------------------------------------------
 // L lanes to a row of up to SHORT_U chunks a lane and up to SHORT_TOP alternatives, all of it in registers: 32 / L rows share a
 // warp's instructions for what comes after the logits (joining the sums, ranking, logarithms), which are most of
-// a short row's work and bound it: 16384 x 1000 f16 in 15.9 us with top 5 (2.1 TB/s), 10.6 without.
+// a short row's work and bound it: 16384 x 1000 f16 in 14.9 us with top 5 (2.2 TB/s), 10.0 without.
 constexpr int SHORT_U = 8, SHORT_TOP = 8, SHORT_KEYS = 32;
 
 template <int L, typename V, typename F> __device__ __forceinline__ V group_reduce(V v, F f) {
@@ -672,7 +672,7 @@ template <int L, typename V, typename F> __device__ __forceinline__ V group_redu
     return v;
 }
 
-template <typename T, int L> __global__ void __launch_bounds__(128, 6) k_token_logprobs_short(const LogprobArgs p) {
+template <typename T, int L> __global__ void __launch_bounds__(128, 7) k_token_logprobs_short(const LogprobArgs p) {
     TB_GRID_DEP_ENTRY();
     constexpr int E = 16 / sizeof(T), U = SHORT_U, G = 32 / L;
     __shared__ unsigned long long found[4][G][SHORT_KEYS];
@@ -794,8 +794,8 @@ template <typename T> int launch_logprobs(tb_ctx* ctx, LogprobArgs p) {
     // within lp_steps() steps. Measured with 1 / 2 / 4 / 8 warps, us: 8192 x 2048 bf16 top 5 18.7 / 25.7 / 47 / 88, 4096 x 32000 60 / 63 / 65 /
     // 77, 1000 x 16000 22.8 / 16.3 / 13.7 / 17.6, 777 x 30001 f32 46 / 27.8 / 19.9 / 23.0.
     // Short rows share warps where they fill the GPU that way, or need no alternatives (else a warp to a row has the shorter
-    // chain, and finds more of them): 16384 x 1000 f16 top 5 in 15.9 us and 21.0 with a warp each, 16384 x 80 8.7 and
-    // 17.7, 60000 x 10 24.7 and 65.6; 200 x 200 4.7 and 4.0.
+    // chain, and finds more of them): 16384 x 1000 f16 top 5 in 14.9 us and 21.0 with a warp each, 16384 x 80 7.2 and
+    // 17.7, 60000 x 10 14.2 and 65.6; 200 x 200 4.7 and 4.0.
     const int lanes = chunks <= 4 * SHORT_U && p.top <= 4 ? 4 : chunks <= 8 * SHORT_U ? 8 : chunks <= 16 * SHORT_U ? 16 : 32;
     if (chunks <= lanes * SHORT_U && p.top <= SHORT_TOP && (p.top == 0 || p.rows * lanes / 32 >= 8 * ctx->sm_count)) {
         auto run = [&](auto n) {
