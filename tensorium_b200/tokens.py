@@ -92,13 +92,19 @@ def _vector(ctx, t, name, dtype, n):
     raise ValueError(f"{name}: stride {t.stride(0)}, 1 is wanted")
 
 
+def _torch_stream(ctx):
+    """The context's stream as torch's. ExternalStream(0) is not the legacy default stream: without an address
+    torch makes a stream of its own."""
+    raw = ctx.raw_stream
+    return torch.cuda.ExternalStream(raw, device=ctx.torch_device) if raw else torch.cuda.default_stream(ctx.torch_device)
+
+
 def _empty(ctx, shapes, dtypes, inputs):
     """New tensors for results. Where the calling thread's current torch stream is not the context's, they
     are allocated on the context's, and the inputs' memory is kept until it has passed this call."""
-    raw = ctx.raw_stream
-    if raw == _current_stream(ctx.device):
+    if ctx.raw_stream == _current_stream(ctx.device):
         return [inputs[0].new_empty(s, dtype=d) for s, d in zip(shapes, dtypes)]
-    stream = torch.cuda.ExternalStream(raw, device=ctx.torch_device)
+    stream = _torch_stream(ctx)
     for t in inputs:
         if t is not None:
             t.record_stream(stream)
