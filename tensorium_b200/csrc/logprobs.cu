@@ -378,22 +378,22 @@ __device__ __forceinline__ void write_row(const LogprobArgs& p, int64_t row, con
     if (lane < p.top) log.write_top(p, row, lane, list);
 }
 
-// The sums of one thread: against a reference of its own, an earlier logit, moved only when a logit is
-// 2^40 above it. The sums are floating point, so nothing is lost below that, and most steps need no new
-// maximum.
+// The sums of one thread, against the largest of its logits so far: that one's term is 2^0 = 1 exactly, so the sum of
+// exponentials is never below 1, and no t 2^t is larger than the entropy's own terms. (A reference that may lag the maximum saves
+// most of the raises, but the sum of t 2^t is then a difference of larger numbers: with a lag of up to 2^40 the entropy of
+// rows sure of their token was off by 6e-7 (rms) instead of 1e-7, and some of their log probabilities were above 0.)
 struct Running {
-    float ref = -INFINITY, max = -INFINITY;
+    float max = -INFINITY;
     F2 z = {0.f, 0.f}, s = {0.f, 0.f};
     int bad = 0;
     // before logits up to m (NaN: one of them is) are added
-    __device__ __forceinline__ void raise(float m, float c, float margin) {
-        max = fmaxf(max, m);
-        if (!(m <= __fadd_rn(ref, margin))) {
+    __device__ __forceinline__ void raise(float m, float c) {
+        if (!(m <= max)) {
             bad |= !(m < INFINITY);
-            const float d = fmaxf(__fmul_rn(__fsub_rn(ref, m), c), EXP_FLOOR), f = exp2_fast(d);
+            const float d = fmaxf(__fmul_rn(__fsub_rn(max, m), c), EXP_FLOOR), f = exp2_fast(d);
             s = {__fmul_rn(fmaf(z.x, d, s.x), f), __fmul_rn(fmaf(z.y, d, s.y), f)};
             z = {__fmul_rn(z.x, f), __fmul_rn(z.y, f)};
-            ref = fmaxf(ref, m);
+            max = fmaxf(max, m);
         }
     }
     // CLAMP: masked logits may be among them; t is kept at EXP_FLOOR there, where 2^t is 0
@@ -403,7 +403,7 @@ struct Running {
         Chunk<T>::get(raw, f);
 #pragma unroll
         for (int e = 0; e < E / 2; ++e) {
-            F2 t = mul2(add2(f[e], {-ref, -ref}), {c, c});
+            F2 t = mul2(add2(f[e], {-max, -max}), {c, c});
             if (CLAMP) t = {fmaxf(t.x, EXP_FLOOR), fmaxf(t.y, EXP_FLOOR)};
             const F2 q = {exp2_fast(t.x), exp2_fast(t.y)};
             z = add2(z, q);
@@ -427,12 +427,7 @@ struct Running {
         for (int u = 0; u < N; ++u)
             if (u < n) add<T, true>(raw[u], c);
     }
-    // against the thread's true maximum
-    __device__ __forceinline__ Sums sums(float c) const {
-        const float d = fmaxf(__fmul_rn(__fsub_rn(ref, max), c), EXP_FLOOR), f = exp2_fast(d);
-        const float zz = __fadd_rn(z.x, z.y), ss = __fadd_rn(s.x, s.y);
-        return {max, __fmul_rn(zz, f), __fmul_rn(fmaf(zz, d, ss), f), bad};
-    }
+    __device__ __forceinline__ Sums sums() const { return {max, __fadd_rn(z.x, z.y), __fadd_rn(s.x, s.y), bad}; }
 };
 
 // The largest float below the value of a bound's key, so that `logit > limit_of(bound)` lets in equal logits
@@ -504,7 +499,7 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? (AHEAD ? 6 
     const Row<T> r(x, p.vocab);
     const int chunks = r.chunks(), per = NW == 1 ? chunks : (int)(((int64_t)chunks + p.splits - 1) / p.splits);
     const int begin = (int)min((int64_t)chunks, (int64_t)split * per), stop = min(chunks, begin + per);
-    const float c = __fmul_rn(LOG2E, p.inv_t), margin = __fdiv_rn(40.f, c);
+    const float c = __fmul_rn(LOG2E, p.inv_t);
 
     Given given;
     if (warp == 0) given.read(p, row, x);
@@ -529,10 +524,10 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? (AHEAD ? 6 
         }
         const float m = Chunk<T>::vmax(raw);
         if (p.top) group_max[steps][tid] = Elem<T>::put(m);  // exact: m is one of the logits
-        a.raise(m, c, margin);
+        a.raise(m, c);
         a.template step<T>(raw, (stop - v0 + NT - 1) / NT, c, !whole, clamp);
     }
-    Sums w = join_warp(a.sums(c), c);
+    Sums w = join_warp(a.sums(), c);
     unsigned long long list = 0;
     if (NW > 1 && lane == 0) sh.sums[warp] = w;
     if (p.top) {
@@ -703,10 +698,10 @@ template <typename T, int L> __global__ void __launch_bounds__(128, 7) k_token_l
 
     const float own = Chunk<T>::vmax(raw);  // NaN if one of the lane's is
     Running a;
-    a.max = group_reduce<L>(own, max_nan);
-    a.bad = !(a.max < INFINITY);
-    a.ref = a.bad ? 0.f : a.max;
-    bool clamp = __any_sync(0xffffffffu, a.max == -INFINITY);
+    const float most = group_reduce<L>(own, max_nan);
+    a.bad = !(most < INFINITY);
+    a.max = a.bad ? 0.f : most;
+    bool clamp = __any_sync(0xffffffffu, most == -INFINITY);
 #pragma unroll
     for (int pass = 0; pass < 2; ++pass) {
 #pragma unroll
@@ -722,7 +717,7 @@ template <typename T, int L> __global__ void __launch_bounds__(128, 7) k_token_l
         a.z = a.s = {0.f, 0.f};
     }
     const auto add = [](float v, float w) { return __fadd_rn(v, w); };
-    const Sums w = {a.max, group_reduce<L>(__fadd_rn(a.z.x, a.z.y), add), group_reduce<L>(__fadd_rn(a.s.x, a.s.y), add), a.bad};
+    const Sums w = {most, group_reduce<L>(__fadd_rn(a.z.x, a.z.y), add), group_reduce<L>(__fadd_rn(a.s.x, a.s.y), add), a.bad};
     const RowLog log(p, w);
     if (gl == 0 && active) log.write(p, row, given);
     if (p.top == 0) return;
