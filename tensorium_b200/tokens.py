@@ -20,10 +20,22 @@ import torch
 from ._lib import ACT, BF16_ELEM, F16_ELEM, F32_ELEM, check, lib
 from .context import Context
 
+
+class _NoFast:
+    """Stands for the extension where it was not built: no call is plain, all go through Python (10 to 18 us of
+    host time instead of 5 to 7, the same kernels and results)."""
+
+    @staticmethod
+    def int8_connected(*args):
+        return None
+
+    token_logprobs = token_logprobs_backward = int8_connected
+
+
 try:
     from . import _tokens_fast as _fast  # ordinary calls, checked and allocated outside Python
-except ImportError as e:
-    raise ImportError(f"{e}: build it with `python -m tensorium_b200.build`") from e
+except ImportError:
+    _fast = _NoFast
 
 _current_stream = torch._C._cuda_getCurrentRawStream
 _ELEM = {torch.float32: F32_ELEM, torch.bfloat16: BF16_ELEM, torch.float16: F16_ELEM}
