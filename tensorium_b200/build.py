@@ -12,10 +12,12 @@ from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
+import importlib.metadata
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -24,7 +26,19 @@ CSRC = PKG / "csrc"
 OBJ = PKG / "_build"
 LIB = PKG / "libtensorium_b200.so"
 FAST_SRC = PKG / "bind" / "tokens_fast.cpp"
-FAST = PKG / "_tokens_fast.so"  # Python extension over the library (see its source)
+
+
+def _fast_path() -> Path:
+    """The Python extension over the library (see its source). It is bound to one Python's and one torch's C++ ABI, so both
+    are in its name: after a change of either it is neither loaded nor up to date."""
+    try:
+        version = importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:
+        version = "none"
+    return PKG / f"_tokens_fast.{sysconfig.get_config_var('SOABI')}.torch-{version}.so"
+
+
+FAST = _fast_path()
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 # --fmad=false: no silent a*b+c contraction; every FMA on the path is an explicit fmaf, so the
@@ -73,8 +87,6 @@ def _compile(src: Path, verbose: bool, extra) -> Path:
 def _build_fast(force: bool, verbose: bool) -> None:
     if not force and not _stale(FAST, [FAST_SRC, LIB]):
         return
-    import sysconfig
-
     import torch
     t = Path(torch.__file__).resolve().parent
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",

@@ -13,11 +13,13 @@ written on another one have to be finished or waited for there first.
 """
 from __future__ import annotations
 
+import importlib.util
 from typing import Optional
 
 import torch
 
 from ._lib import ACT, BF16_ELEM, F16_ELEM, F32_ELEM, check, lib
+from .build import FAST
 from .context import Context
 
 
@@ -32,10 +34,19 @@ class _NoFast:
     token_logprobs = token_logprobs_backward = int8_connected
 
 
-try:
-    from . import _tokens_fast as _fast  # ordinary calls, checked and allocated outside Python
-except ImportError:
-    _fast = _NoFast
+def _load_fast():
+    if not FAST.exists():
+        return _NoFast
+    spec = importlib.util.spec_from_file_location(f"{__package__}._tokens_fast", FAST)
+    try:
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+    except ImportError:
+        return _NoFast
+    return module
+
+
+_fast = _load_fast()  # ordinary calls, checked and allocated outside Python
 
 _current_stream = torch._C._cuda_getCurrentRawStream
 _ELEM = {torch.float32: F32_ELEM, torch.bfloat16: BF16_ELEM, torch.float16: F16_ELEM}

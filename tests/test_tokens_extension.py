@@ -54,6 +54,40 @@ def test_library_builds_without_the_extension(monkeypatch, tmp_path, capsys, why
     assert B.build() == B.LIB and not fast.exists()
 
 
+def test_another_torch_or_python_has_another_extension(monkeypatch):
+    """One that was built for another C++ ABI is not loaded, nor taken for up to date."""
+    assert B._fast_path() == B.FAST
+    seen = {B.FAST}
+    monkeypatch.setattr(B.importlib.metadata, "version", lambda name: "99.1.0+cu990")
+    seen.add(B._fast_path())
+    monkeypatch.setattr(B.sysconfig, "get_config_var", lambda name: "cpython-399-x86_64-linux-gnu")
+    seen.add(B._fast_path())
+    assert len(seen) == 3
+
+    def none(name):
+        raise B.importlib.metadata.PackageNotFoundError(name)
+
+    monkeypatch.setattr(B.importlib.metadata, "version", none)
+    assert B._fast_path() not in seen
+
+
+@pytest.mark.parametrize("content", [None, b"", b"not a library"])
+def test_import_with_another_torchs_extension(tmp_path, content):
+    """Only the file of this Python and torch counts, and one that does not load is passed over."""
+    fast = tmp_path / "_tokens_fast.so"
+    if content is not None:
+        fast.write_bytes(content)
+    r = python(f"""
+import pathlib
+from tensorium_b200 import build
+build.FAST = pathlib.Path({str(fast)!r})
+import tensorium_b200.layers, tensorium_b200.net
+from tensorium_b200 import tokens
+assert tokens._fast is tokens._NoFast
+""")
+    assert r.returncode == 0, r.stderr
+
+
 @pytest.mark.gpu
 def test_same_results_without_the_extension(ctx, monkeypatch):
     from tensorium_b200 import tokens as K
