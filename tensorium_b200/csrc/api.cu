@@ -302,11 +302,14 @@ int tb_init(int64_t device, const tb_options* opts, tb_ctx** out) {
     cudaEventCreateWithFlags(&c->join, cudaEventDisableTiming);
     e = cudaMalloc(&c->d_status, sizeof(int) * 4);
     if (e != cudaSuccess) { cudaStreamDestroy(c->own_stream); delete c; return cuda_fail(e, "cudaMalloc(status)"); }
-    cudaMemset(c->d_status, 0, sizeof(int) * 4);
     c->tile_cnt_len = 1 << 16;
     e = cudaMalloc(&c->tile_cnt, sizeof(int) * c->tile_cnt_len);
     if (e != cudaSuccess) { cudaFree(c->d_status); cudaStreamDestroy(c->own_stream); delete c; return cuda_fail(e, "cudaMalloc(tile counters)"); }
-    cudaMemset(c->tile_cnt, 0, sizeof(int) * c->tile_cnt_len);
+    // waited for: launches may go to any stream from here on
+    e = cudaMemsetAsync(c->d_status, 0, sizeof(int) * 4, c->own_stream);
+    if (e == cudaSuccess) e = cudaMemsetAsync(c->tile_cnt, 0, sizeof(int) * c->tile_cnt_len, c->own_stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(c->own_stream);
+    if (e != cudaSuccess) { cudaFree(c->d_status); cudaFree(c->tile_cnt); cudaStreamDestroy(c->own_stream); delete c; return cuda_fail(e, "cudaMemset(tile counters)"); }
     int64_t ws = (opts && opts->workspace_bytes > 0) ? opts->workspace_bytes : (64ll << 20);
     int r = ensure_workspace(c, (size_t)ws);
     if (r != TB_OK) { cudaFree(c->d_status); cudaStreamDestroy(c->own_stream); delete c; return r; }
@@ -339,14 +342,10 @@ void* tb_get_stream(tb_ctx* ctx) { return ctx ? (void*)ctx->stream : nullptr; }
 
 int tb_sync(tb_ctx* ctx) {
     TB_ENTER(ctx);
-    TB_CHECK_CUDA(cudaStreamSynchronize(ctx->stream));
     int st = 0;
-    TB_CHECK_CUDA(cudaMemcpy(&st, ctx->d_status, sizeof(int), cudaMemcpyDeviceToHost));
-    if (st != 0) {
-        cudaMemset(ctx->d_status, 0, sizeof(int));
-        cudaMemset(ctx->tile_cnt, 0, sizeof(int) * ctx->tile_cnt_len);  // a kernel that gave up leaves counts behind
-        return fail(TB_ERR_DEVICE, "a kernel reported device status %d", st);
-    }
+    const int r = take_status(ctx, &st);
+    if (r != TB_OK) return r;
+    if (st != 0) return fail(TB_ERR_DEVICE, "a kernel reported device status %d", st);
     return TB_OK;
 }
 

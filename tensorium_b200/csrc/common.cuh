@@ -9,30 +9,11 @@
 #include <cstdarg>
 #include <utility>
 
-#include "../../include/tensorium_b200.h"
-
-struct tb_ctx {
-    int device = 0;
-    cudaStream_t stream = nullptr;      // current launch stream
-    cudaStream_t own_stream = nullptr;  // stream created by tb_init
-    void* ws = nullptr;                 // split-K / scratch workspace
-    size_t ws_bytes = 0;
-    int* d_status = nullptr;            // device status word (kernels report errors here)
-    int64_t math_mode = TB_MATH_FP32;
-    int sm_count = 148;
-    int max_smem_optin = 0;
-    cudaEvent_t fork = nullptr, join = nullptr;  // order own_stream work with `stream`
-    int* tile_cnt = nullptr;                      // split-K arrival counters (zeroed, self-resetting)
-    int64_t tile_cnt_len = 0;
-    int pdl = 0;  // launches through tbi::launch may overlap the previous kernel's tail (set while
-                  // a network forward is captured)
-};
+#include "ctx.cuh"
 
 namespace tbi {
 
 void set_error(const char* fmt, ...);
-int fail(int code, const char* fmt, ...);
-int cuda_fail(cudaError_t e, const char* what);
 // Make ctx's device current on this thread; returns TB_OK or an error code.
 int enter(tb_ctx* ctx);
 // Ensure the workspace holds at least `bytes` (may allocate; not capture-safe).
@@ -91,12 +72,6 @@ inline unsigned grid_for(int64_t n, int threads, int sm_count, int per_thread = 
 bool act_supported(int64_t act);
 
 }  // namespace tbi
-
-#define TB_CHECK_CUDA(call)                                              \
-    do {                                                                  \
-        cudaError_t _e = (call);                                          \
-        if (_e != cudaSuccess) return tbi::cuda_fail(_e, #call);          \
-    } while (0)
 
 #define TB_ENTER(ctx)                                                    \
     do {                                                                  \

@@ -584,6 +584,8 @@ int tb_net_destroy(tb_net* net) {
     if (net->fork_ev) cudaEventDestroy(net->fork_ev);
     if (net->join_ev) cudaEventDestroy(net->join_ev);
     if (net->side) cudaStreamDestroy(net->side);
+    auto& cnts = net->ctx->side_cnts;
+    cnts.erase(std::remove(cnts.begin(), cnts.end(), std::make_pair(net->side_cnt, net->side_cnt_len)), cnts.end());
     for (float* p : net->allocs) cudaFree(p);
     delete net;
     return TB_OK;
@@ -1065,7 +1067,8 @@ int tb_net_finalize(tb_net* net, int64_t math_mode) {
                 float* c = alloc(std::max<int64_t>(net->side_cnt_len, 1));
                 if (!c) return err;
                 net->side_cnt = reinterpret_cast<int*>(c);
-                TB_CHECK_CUDA(cudaMemset(net->side_cnt, 0, (size_t)std::max<int64_t>(net->side_cnt_len, 1) * sizeof(int)));
+                TB_CHECK_CUDA(cudaMemsetAsync(net->side_cnt, 0, (size_t)std::max<int64_t>(net->side_cnt_len, 1) * sizeof(int), net->ctx->stream));
+                net->ctx->side_cnts.emplace_back(net->side_cnt, net->side_cnt_len);
             }
         }
         bool ok = !net->nhwc && math_mode == TB_MATH_FP32 && !off;
