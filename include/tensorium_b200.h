@@ -24,7 +24,8 @@
  *     tb_int8_gemm (partial sums: 1 KB a token and SM, 20 MB at most) and tb_token_logprobs_fwd
  *     (parts of rows: 272 bytes each, under 1 MB for the few rows that are split, more only with
  *     over 114688 float or 262144 16-bit columns). Growth is refused (TB_ERR_STATE) while the stream is being
- *     captured into a CUDA graph; reserve first with tb_workspace_reserve.
+ *     captured into a CUDA graph; reserve first with tb_workspace_reserve. A workspace that a captured
+ *     graph may use is kept until tb_shutdown, so graphs stay valid when later calls make it grow.
  */
 #ifndef TENSORIUM_B200_H
 #define TENSORIUM_B200_H

@@ -40,26 +40,6 @@ int enter(tb_ctx* ctx) {
     return TB_OK;
 }
 
-int ensure_workspace(tb_ctx* ctx, size_t bytes) {
-    if (bytes <= ctx->ws_bytes) return TB_OK;
-    cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-    cudaStreamIsCapturing(ctx->stream, &cs);
-    if (cs != cudaStreamCaptureStatusNone)
-        return fail(TB_ERR_STATE, "workspace of %zu bytes needed during stream capture (have %zu); "
-                    "call tb_workspace_reserve first", bytes, ctx->ws_bytes);
-    // the old buffer may still be read by queued work on this stream
-    cudaError_t e = cudaStreamSynchronize(ctx->stream);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaStreamSynchronize");
-    if (ctx->ws) cudaFree(ctx->ws);
-    ctx->ws = nullptr;
-    ctx->ws_bytes = 0;
-    size_t want = round_up((int64_t)bytes, 1 << 20);
-    e = cudaMalloc(&ctx->ws, want);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaMalloc(workspace)");
-    ctx->ws_bytes = want;
-    return TB_OK;
-}
-
 int check_launch(const char* what) {
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, what);
@@ -323,6 +303,7 @@ int tb_shutdown(tb_ctx* ctx) {
     if (ctx->own_stream) cudaStreamSynchronize(ctx->own_stream);
     if (ctx->stream && ctx->stream != ctx->own_stream) cudaStreamSynchronize(ctx->stream);
     if (ctx->ws) cudaFree(ctx->ws);
+    for (void* p : ctx->ws_kept) cudaFree(p);
     if (ctx->d_status) cudaFree(ctx->d_status);
     if (ctx->tile_cnt) cudaFree(ctx->tile_cnt);
     if (ctx->own_stream) cudaStreamDestroy(ctx->own_stream);

@@ -16,8 +16,6 @@ namespace tbi {
 void set_error(const char* fmt, ...);
 // Make ctx's device current on this thread; returns TB_OK or an error code.
 int enter(tb_ctx* ctx);
-// Ensure the workspace holds at least `bytes` (may allocate; not capture-safe).
-int ensure_workspace(tb_ctx* ctx, size_t bytes);
 // Check the last launch.
 int check_launch(const char* what);
 // Keep the stream busy for about `us` microseconds (a bounded sleep on the GPU timer), so that the

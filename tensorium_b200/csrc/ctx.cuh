@@ -15,6 +15,8 @@ struct tb_ctx {
     cudaStream_t own_stream = nullptr;  // stream created by tb_init
     void* ws = nullptr;                 // split-K / scratch workspace
     size_t ws_bytes = 0;
+    bool ws_in_graph = false;           // a captured graph may hold ws's address
+    std::vector<void*> ws_kept;         // outgrown workspaces that graphs may hold
     int* d_status = nullptr;            // device status word (kernels report errors here)
     int64_t math_mode = TB_MATH_FP32;
     int sm_count = 148;
@@ -31,6 +33,9 @@ namespace tbi {
 
 int fail(int code, const char* fmt, ...);
 int cuda_fail(cudaError_t e, const char* what);
+// The workspace holds at least `bytes` from here on (may allocate, except during capture). A workspace that a captured graph
+// may use is kept until the context ends, so that the graph can be replayed after a growth.
+int ensure_workspace(tb_ctx* ctx, size_t bytes);
 // The device status word, once the work on ctx's stream has ended. A kernel that gave up leaves its arrival counters as they
 // were: where there is a status, it and every counter are 0 again before this returns.
 int take_status(tb_ctx* ctx, int* status);

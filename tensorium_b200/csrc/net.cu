@@ -1112,6 +1112,7 @@ int tb_net_forward(tb_net* net, const float* x, int64_t use_graph) {
         // FP32 plan ~7% (dependent CTAs held resident beside the multi-wave FP32 grids).
         static const bool pdl = getenv("TB_PDL") != nullptr && atoi(getenv("TB_PDL")) != 0;
         ctx->pdl = pdl ? 1 : 0;
+        ctx->ws_in_graph = true;
         int r = run_all(net, x);
         ctx->pdl = 0;
         cudaGraph_t g = nullptr;

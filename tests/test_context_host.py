@@ -43,6 +43,7 @@ cudaError_t cudaStreamIsCapturing(cudaStream_t, cudaStreamCaptureStatus* c) {
     *c = capturing ? cudaStreamCaptureStatusActive : cudaStreamCaptureStatusNone;
     return cudaSuccess;
 }
+cudaError_t cudaGetLastError() { return cudaSuccess; }
 cudaError_t cudaMalloc(void** p, size_t n) {
     if (n > device_left) return cudaErrorMemoryAllocation;
     *p = malloc(n);
@@ -118,3 +119,81 @@ def test_a_clear_that_fails_is_reported(tmp_path):
     dirty(942);
     CHECK(tbi::take_status(&c, &st) == TB_OK && st == 942 && !left(cnt) && !left(side2));
 ''')
+
+
+WORKSPACE = r'''
+    tb_ctx c;
+    c.stream = (cudaStream_t)5;
+    const size_t MB = 1 << 20;
+    CHECK(tbi::ensure_workspace(&c, 3) == TB_OK && c.ws_bytes == MB && live.size() == 1);
+    void* first = c.ws;
+'''
+
+
+def test_a_workspace_that_no_graph_uses_is_freed(tmp_path):
+    run(tmp_path, WORKSPACE + r'''
+    CHECK(tbi::ensure_workspace(&c, MB) == TB_OK && c.ws == first);
+    calls.clear();
+    CHECK(tbi::ensure_workspace(&c, MB + 1) == TB_OK && c.ws_bytes == 2 * MB && c.ws != first);
+    CHECK(calls == "sync:5 free:0 " && live.size() == 1 && live.count(c.ws));
+''')
+
+
+def test_a_workspace_that_a_graph_may_use_is_kept(tmp_path):
+    """A captured call holds the address; the graph is replayed after other calls have made the workspace grow."""
+    run(tmp_path, WORKSPACE + r'''
+    capturing = 1;
+    CHECK(tbi::ensure_workspace(&c, 100) == TB_OK);
+    CHECK(tbi::ensure_workspace(&c, 2 * MB) == TB_ERR_STATE && c.ws == first);
+    capturing = 0;
+    CHECK(tbi::ensure_workspace(&c, 2 * MB) == TB_OK && c.ws != first);
+    CHECK(live.count(first) && c.ws_kept.size() == 1 && c.ws_kept[0] == first);
+    // the new one is in no graph yet
+    void* second = c.ws;
+    CHECK(tbi::ensure_workspace(&c, 4 * MB) == TB_OK && !live.count(second) && live.size() == 2);
+''')
+
+
+def test_a_growth_that_fails_leaves_the_workspace(tmp_path):
+    run(tmp_path, WORKSPACE + r'''
+    device_left = 0;
+    CHECK(tbi::ensure_workspace(&c, 5 * MB) == TB_ERR_OOM);
+    CHECK(c.ws == first && c.ws_bytes == MB && live.count(first));
+    device_left = ~(size_t)0;
+    fail_at = count;  // the wait for queued work fails
+    CHECK(tbi::ensure_workspace(&c, 5 * MB) == TB_ERR_CUDA);
+    CHECK(c.ws == first && c.ws_bytes == MB && live.count(first) && live.size() == 1);
+''')
+
+
+@pytest.mark.gpu
+def test_a_graph_is_replayed_after_the_workspace_has_grown():
+    import torch
+
+    import tokens_ref as R
+    from tensorium_b200 import Context
+    from tensorium_b200 import tokens as K
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(40, 512, device="cuda", generator=g)
+    w = torch.randint(-127, 128, (300, 512), device="cuda", generator=g, dtype=torch.int8)
+    sw = torch.full((300,), 1e-3, device="cuda")
+    out = torch.empty(40, 300, device="cuda")
+    side = torch.cuda.Stream()
+    with Context(0, workspace_bytes=32 << 20, use_torch_stream=False) as c:
+        c.set_stream(side)
+        side.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            K.int8_connected(c, x, w, sw, out=out)
+        c.reserve(256 << 20)
+        others = [torch.full((8 << 20,), 3.0, device="cuda") for _ in range(8)]  # would take the freed memory
+        torch.cuda.synchronize()
+        x.mul_(2).add_(0.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        f64 = lambda t: t.double().cpu().numpy()
+        codes, scales = R.quantize(f64(x))
+        ref, off = R.product(codes, scales, f64(w), f64(sw), None, "linear", "float32")
+        assert (abs(f64(out) - ref) <= off).all()
+        assert all((t == 3).all() for t in others)
+        del graph
