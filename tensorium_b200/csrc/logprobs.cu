@@ -469,6 +469,7 @@ constexpr int KEYS = 64;  // candidates that are ranked against one another
 
 template <int NW> struct RowShared {
     unsigned long long keys[NW][32];
+    uint32_t maxima[NW][32];
     Sums sums[NW];
     unsigned long long found[KEYS], ranked[32];
     unsigned long long bound;
@@ -534,7 +535,7 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32, NW == 1 ? (AHEAD ? 6 
         uint32_t o = ordered(a.max);
         if constexpr (NW > 1) {
             o = sort32(o, lane);
-            o = merge_warps<NW>(o, reinterpret_cast<uint32_t (*)[32]>(sh.keys), warp, lane);
+            o = merge_warps<NW>(o, sh.maxima, warp, lane);
             if (warp == 0) {
                 o = __shfl_sync(0xffffffffu, o, p.top - 1);
                 if (lane == 0) sh.bound = unordered(o) > -INFINITY ? (unsigned long long)o << 32 : 0;
