@@ -1,5 +1,5 @@
-// elem.cuh -- the element types of the token operators (TB_F32, TB_BF16, TB_F16): conversions and
-// 16-byte accesses that never touch memory outside a row.
+// elem.cuh -- the element types of the token operators (TB_F32, TB_BF16, TB_F16): conversions, dispatch on them, and the
+// operators' launches.
 #pragma once
 #include "common.cuh"
 
@@ -22,10 +22,9 @@ template <> struct Elem<__half> {
     static __device__ __forceinline__ __half put(float v) { return __float2half_rn(v); }
 };
 
-// 16 bytes of elements
-template <typename T> struct __align__(16) Vec {
+// elements in 16 bytes
+template <typename T> struct Vec {
     static constexpr int N = 16 / sizeof(T);
-    T e[N];
 };
 
 inline bool elem_type_ok(int64_t t) { return t == TB_F32 || t == TB_BF16 || t == TB_F16; }

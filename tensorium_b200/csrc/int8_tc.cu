@@ -110,32 +110,35 @@ constexpr int I8S_SMEM = 216 * 1024;
 struct StreamArgs {
     int bt;        // tokens of a tile: a multiple of 16 up to 128
     int stages;
-    int tiles_m, ktiles;
-    int sk_tiles;  // tiles 0 .. sk_tiles - 1 are shared out by units of 128 bytes of k, the others whole
-    int dp_tiles;  // tiles after them
+    int tiles_m, tiles, ktiles;
+    bool share;    // the tiles are shared out by units of 128 bytes of k, else they are taken whole
     int* partial;  // [2 x CTA][bt / 4][128 channels][4 tokens]
     int* counters; // per shared tile: CTAs that have left their sums, left at 0
 };
 
-// A CTA's work in order: its range of the shared tiles' units, then every gridDim.x-th whole tile.
+// A CTA's work in order: its range of the shared tiles' units, or every gridDim.x-th whole tile.
 struct StreamWork {
-    int u, end, next, ktiles, tiles, step;
-    int tile, kb, ke;  // the current piece
-    __device__ StreamWork(const StreamArgs& a)
-        : u((int)((int64_t)a.sk_tiles * a.ktiles * blockIdx.x / gridDim.x)),
-          end((int)((int64_t)a.sk_tiles * a.ktiles * (blockIdx.x + 1) / gridDim.x)),
-          next(a.sk_tiles + blockIdx.x), ktiles(a.ktiles), tiles(a.sk_tiles + a.dp_tiles), step(gridDim.x) {}
-    __device__ __forceinline__ bool take() {
-        if (u < end) {
-            tile = u / ktiles;
-            kb = u - tile * ktiles;
-            ke = min(ktiles, kb + end - u);
-            u += ke - kb;
-            return true;
+    bool share;
+    int at, end, step, ktiles;  // unit and end of the range, or tile and number of tiles
+    int tile, kb, ke;           // the current piece
+    __device__ StreamWork(const StreamArgs& a) : share(a.share), at(blockIdx.x), end(a.tiles), step(gridDim.x), ktiles(a.ktiles) {
+        if (share) {
+            const int64_t units = (int64_t)a.tiles * a.ktiles;
+            at = (int)(units * blockIdx.x / gridDim.x);
+            end = (int)(units * (blockIdx.x + 1) / gridDim.x);
         }
-        if (next >= tiles) return false;
-        tile = next, kb = 0, ke = ktiles;
-        next += step;
+    }
+    __device__ __forceinline__ bool take() {
+        if (at >= end) return false;
+        if (share) {
+            tile = at / ktiles;
+            kb = at - tile * ktiles;
+            ke = min(ktiles, kb + end - at);
+            at += ke - kb;
+        } else {
+            tile = at, kb = 0, ke = ktiles;
+            at += step;
+        }
         return true;
     }
 };
@@ -243,7 +246,7 @@ __global__ void __launch_bounds__(I8S_THREADS, 1) k_int8_stream(const __grid_con
     } else {
         grid_dep_wait();  // a_scales
         const int quarter = warp & 3, half = (warp - 2) >> 2, ch = quarter * 32 + lane, et = tid - 64;
-        const int64_t units = (int64_t)g.sk_tiles * g.ktiles;
+        const int64_t units = (int64_t)g.tiles * g.ktiles;
         int n = 0;
         for (StreamWork w(g); w.take(); ++n) {
             const int buf = n & 1, u = n >> 1;
@@ -561,10 +564,10 @@ int launch_stream(tb_ctx* ctx, const Int8Args& p, int64_t y_type, bool early, co
     g.bt = bt;
     g.stages = (int)std::min<int64_t>(I8S_MAX_STAGES, (I8S_SMEM - 1024) / (I8_W_BYTES + bt * I8_BK));
     g.tiles_m = (int)tiles_m;
+    g.tiles = (int)tiles;
     g.ktiles = (int)ceil_div(p.k, I8_BK);
-    g.sk_tiles = plan.share ? (int)tiles : 0;
-    g.dp_tiles = (int)(tiles - g.sk_tiles);
-    if (g.sk_tiles) {
+    g.share = plan.share;
+    if (g.share) {
         const size_t need = scratch + (size_t)plan.grid * 2 * bt * 128 * 4;
         if (need > ctx->ws_bytes && scratch) return fail(TB_ERR_STATE, "int8 product: workspace not reserved");
         if ((r = ensure_workspace(ctx, need)) != TB_OK) return r;
