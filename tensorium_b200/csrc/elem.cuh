@@ -6,6 +6,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <initializer_list>
+
 namespace tbi {
 
 template <typename T> struct Elem;
@@ -29,6 +31,12 @@ template <typename T> struct Vec {
 
 inline bool elem_type_ok(int64_t t) { return t == TB_F32 || t == TB_BF16 || t == TB_F16; }
 inline size_t elem_size(int64_t t) { return t == TB_F32 ? 4 : 2; }
+// whether each address (null too) is a multiple of n bytes
+inline bool aligned_to(size_t n, std::initializer_list<const void*> addresses) {
+    for (const void* p : addresses)
+        if ((uintptr_t)p % n) return false;
+    return true;
+}
 
 // launch() that lets the kernel be scheduled while the one before it on the stream still runs: its set-up hides the
 // launch's latency, and it waits for that kernel's end itself (TB_GRID_DEP_ENTRY) before it reads or writes

@@ -377,7 +377,7 @@ int check_quantize(int64_t rows, int64_t cols, const void* x, int64_t x_type, in
 
 // what the product asks of everything but its a operand
 int check_product(int64_t m, int64_t n, int64_t k, const int8_t* w, int64_t w_stride, const float* w_scales,
-                  int64_t act, void* y, int64_t y_type, int64_t y_stride) {
+                  const float* bias, int64_t act, void* y, int64_t y_type, int64_t y_stride) {
     if (m < 0 || n < 0 || k <= 0 || m > MAX_DIM || n > MAX_DIM) return fail(TB_ERR_INVALID, "int8 product: bad shape");
     if (k > INT8_MAX_K) return fail(TB_ERR_UNSUPPORTED, "int8 product: k over %lld can overflow the int32 sum", (long long)INT8_MAX_K);
     if (!act_supported(act)) return fail(TB_ERR_UNSUPPORTED, "int8 product: activation %lld not supported", (long long)act);
@@ -385,6 +385,7 @@ int check_product(int64_t m, int64_t n, int64_t k, const int8_t* w, int64_t w_st
     if (m == 0 || n == 0) return TB_OK;
     if (!w || !w_scales || !y) return fail(TB_ERR_INVALID, "int8 product: null pointer");
     if ((uintptr_t)y % elem_size(y_type)) return fail(TB_ERR_INVALID, "int8 product: misaligned output");
+    if (!aligned_to(4, {w_scales, bias})) return fail(TB_ERR_INVALID, "int8 product: misaligned scales or bias");
     if (!aligned16(w) || w_stride % 16) return fail(TB_ERR_INVALID, "int8 product: w and its stride have to be multiples of 16 bytes");
     if ((n > 1 && w_stride < k) || (m > 1 && y_stride < n)) return fail(TB_ERR_INVALID, "int8 product: row stride below the row's length");
     return TB_OK;
@@ -404,6 +405,7 @@ int tb_quantize_rows(tb_ctx* ctx, int64_t rows, int64_t cols, const void* x, int
     if (r != TB_OK) return r;
     if (rows == 0) return TB_OK;
     if (!codes || !scales) return fail(TB_ERR_INVALID, "quantize: null pointer");
+    if (!aligned_to(4, {scales})) return fail(TB_ERR_INVALID, "quantize: misaligned scales");
     if (rows > 1 && code_stride < cols) return fail(TB_ERR_INVALID, "quantize: row stride below the row's length");
     return quantize_rows(ctx, rows, cols, x, x_type, x_stride, codes, code_stride, scales);
 }
@@ -412,10 +414,11 @@ int tb_int8_gemm(tb_ctx* ctx, int64_t m, int64_t n, int64_t k, const int8_t* a, 
                  const float* a_scales, const int8_t* w, int64_t w_stride, const float* w_scales,
                  const float* bias, int64_t activation, void* y, int64_t y_type, int64_t y_stride) {
     TB_ENTER(ctx);
-    int r = check_product(m, n, k, w, w_stride, w_scales, activation, y, y_type, y_stride);
+    int r = check_product(m, n, k, w, w_stride, w_scales, bias, activation, y, y_type, y_stride);
     if (r != TB_OK) return r;
     if (m == 0 || n == 0) return TB_OK;
     if (!a || !a_scales) return fail(TB_ERR_INVALID, "int8 product: null pointer");
+    if (!aligned_to(4, {a_scales})) return fail(TB_ERR_INVALID, "int8 product: misaligned scales or bias");
     if (!aligned16(a) || a_stride % 16) return fail(TB_ERR_INVALID, "int8 product: a and its stride have to be multiples of 16 bytes");
     if (m > 1 && a_stride < k) return fail(TB_ERR_INVALID, "int8 product: row stride below the row's length");
     const Int8Args p{m, n, k, a, a_stride, a_scales, w, w_stride, w_scales, bias, (int)activation, y, y_stride};
@@ -427,7 +430,7 @@ int tb_int8_connected_fwd(tb_ctx* ctx, int64_t m, int64_t n, int64_t k, const vo
                           int64_t x_stride, const int8_t* w, int64_t w_stride, const float* w_scales,
                           const float* bias, int64_t activation, void* y, int64_t y_type, int64_t y_stride) {
     TB_ENTER(ctx);
-    int r = check_product(m, n, k, w, w_stride, w_scales, activation, y, y_type, y_stride);
+    int r = check_product(m, n, k, w, w_stride, w_scales, bias, activation, y, y_type, y_stride);
     if (r != TB_OK) return r;
     if ((r = check_quantize(m, k, x, x_type, x_stride)) != TB_OK) return r;
     if (m == 0 || n == 0) return TB_OK;

@@ -972,6 +972,8 @@ int tb_token_logprobs_fwd(tb_ctx* ctx, int64_t rows, int64_t vocab, const void* 
     if (top > TOP_MAX) return fail(TB_ERR_UNSUPPORTED, "token logprobs: top over %d", TOP_MAX);
     if (rows == 0) return TB_OK;
     if ((tokens && !logprob) || (top && (!top_logprob || !top_token))) return fail(TB_ERR_INVALID, "token logprobs: null pointer");
+    if (!aligned_to(4, {logprob, entropy, lse, row_max, log_sum, top_logprob}) || !aligned_to(8, {tokens, top_token}))
+        return fail(TB_ERR_INVALID, "token logprobs: misaligned pointer");
     LogprobArgs p{rows, vocab, logits, stride, tokens, 1.f / temperature, (int)top, tokens ? logprob : nullptr, entropy, lse, row_max, log_sum, top_logprob, top_token, 0, 1, nullptr, nullptr};
     return elem_dispatch(type, [&](auto t) { return launch_logprobs<decltype(t)>(ctx, p); });
 }
@@ -986,7 +988,8 @@ int tb_token_logprobs_bwd(tb_ctx* ctx, int64_t rows, int64_t vocab, const void* 
     if (rows > 1 && d_stride < vocab) return fail(TB_ERR_INVALID, "token logprobs: row stride below the row's length");
     if (rows == 0) return TB_OK;
     if (!row_max || !log_sum || !dlogits || (g_logprob && !tokens) || (g_entropy && !entropy)) return fail(TB_ERR_INVALID, "token logprobs: null pointer");
-    if ((uintptr_t)dlogits % elem_size(type)) return fail(TB_ERR_INVALID, "token logprobs: misaligned pointer");
+    if ((uintptr_t)dlogits % elem_size(type) || !aligned_to(4, {row_max, log_sum, entropy, g_logprob, g_entropy}) || !aligned_to(8, {tokens}))
+        return fail(TB_ERR_INVALID, "token logprobs: misaligned pointer");
     if (dlogits == logits && rows > 1 && d_stride != stride) return fail(TB_ERR_INVALID, "token logprobs: in place with another row stride");
     const LogprobBwdArgs p{rows, vocab, logits, stride, tokens, 1.f / temperature, row_max, log_sum, entropy, g_logprob, g_entropy, dlogits, d_stride, 1};
     return elem_dispatch(type, [&](auto t) { return launch_bwd<decltype(t)>(ctx, p); });
