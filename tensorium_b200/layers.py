@@ -351,7 +351,7 @@ class TInt8ConnectedLayer(TBaseLayer):
         self.inputs, self.outputs = AInputs, aOutputs
         self.ActivationType = _act(AActivationType)
         self.weights = weights if weights is not None else np.zeros((aOutputs, AInputs), np.float32)
-        self.biases = biases  # float32 [aOutputs] or None
+        self.biases = biases  # [aOutputs] or None; like the weights an array or a tensor
         self._dev = None
 
     def upload(self, ctx: Context = None):
@@ -361,7 +361,10 @@ class TInt8ConnectedLayer(TBaseLayer):
         w = self.weights
         w = w.to(self.ctx.torch_device) if isinstance(w, torch.Tensor) else _dev(self.ctx, w)
         codes, scales = tokens.quantize_rows(self.ctx, w)
-        self._dev = (codes, scales, None if self.biases is None else _dev(self.ctx, self.biases))
+        b = self.biases
+        if b is not None:
+            b = b.detach().to(self.ctx.torch_device, torch.float32) if isinstance(b, torch.Tensor) else _dev(self.ctx, b)
+        self._dev = (codes, scales, b)
 
     def forward(self, state: TNNetState):
         if self._dev is None:
