@@ -427,8 +427,9 @@ int tb_bn_fwd(tb_ctx* ctx, int64_t batch, int64_t channels, int64_t spatial, con
  * (a scale for each token, i.e. row of x, and for each output channel) and what a program reads
  * off its logits. The reference has neither; these entry points are new. Matrices are row-major
  * with a row stride in elements, at least the row's length unless there is one row; x, y and logits
- * are of a TB_* element type and need no alignment beyond their element's. Nothing outside the
- * rows is read or written. Zero rows are a valid call that does nothing. */
+ * are of a TB_* element type and need no alignment beyond their element's; other addresses are multiples
+ * of their element's size too (TB_ERR_INVALID). Nothing outside the rows is read or written. Results do
+ * not overlap inputs, but for dlogits in place. Zero rows are a valid call that does nothing. */
 #define TB_F32  0
 #define TB_BF16 1
 #define TB_F16  2

@@ -160,8 +160,9 @@ int quantize_rows(tb_ctx* ctx, int64_t rows, int64_t cols, const void* x, int64_
 // 64-byte steps of k through a ring of its own (cp.async, read back by the lane that copied it: no barrier), FEW_RING
 // steps ahead and on into the next groups; the int32 partial sums meet in shared memory. A CTA quantizes the
 // tokens for itself while its first weights are on their way, which saves the launch, and the round trip, of
-// a quantizer. 1 to 4 tokens x 4096 x 4096: 7.4 us where the bytes take 2.6, the rest being the launch, the first loads' and the
-// last sums' latency; 4 x 16384 x 4096: 16.4 us (4.1 TB/s).
+// a quantizer. 1 to 4 tokens x 4096 x 4096: 7.0 to 7.3 us where the bytes take 2.6, the rest being the launch, the first loads' and the
+// last sums' latency; 4 x 16384 x 4096: 16.1 us (4.2 TB/s). (Times in this file: in a graph of calls on
+// several weights in turn, larger than L2 together.)
 constexpr int FEW_WARPS = 16, FEW_RING = 6, FEW_THREADS = FEW_WARPS * 32;
 constexpr int FEW_RING_BYTES = FEW_WARPS * FEW_RING * 1024;
 constexpr int FEW_CODES = 96 * 1024;  // most bytes of codes
@@ -335,8 +336,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) k_int8_few(const FewArgs g) {
 
 // Up to 16 tokens whose codes fit, where that is the faster of the two. Measured, us: this one 4.6 + 0.178 a MB of
 // weights + 0.1 a thousand values of x (each CTA quantizes them); the tensor cores 7.5 + 0.155 a MB, 4 more where
-// their tiles are too few to fill the SMs whole. 4096 x 4096: 7.6 and 13 for 4 tokens, 14.4 and 13.6 for 16; 16384 x 4096: 16.4
-// and 17.5 for 4 tokens, 19.0 and 17.8 for 8; 131072 x 4096: 104 and 92 for 1.
+// their tiles are too few to fill the SMs whole. 4096 x 4096: 7.0 and 12.9 for 4 tokens, 13.8 and 13.4 for 16; 16384 x 4096: 16.1
+// and 16.9 for 4 tokens, 18.6 and 17.0 for 8; 131072 x 4096: 103 and 92 for 1.
 bool use_few(const tb_ctx* ctx, int64_t m, int64_t n, int64_t k) {
     if (m > 16 || m * few_pitch(k) > FEW_CODES) return false;
     const double more = 1e-4 * (double)(m * k) + 2.3e-8 * (double)(n * k);

@@ -8,8 +8,9 @@
 // 128-byte swizzled rows; TMA fills zeros past k, m and n, so no size needs padding. int32 sums are
 // exact in any order, which is what lets k be split freely.
 //
-// k_int8_stream: one CTA per SM on tiles of 128 channels x up to 128 tokens. One SM streams from HBM at 43 to 48 GB/s at
-// most (measured, with 5 as with 10 stages in flight), so a few long tiles are shared out by k, to
+// k_int8_stream: one CTA per SM on tiles of 128 channels x up to 128 tokens. One SM takes weights at 58 GB/s at most, with 5 as
+// with 10 stages in flight, and 148 of them at 43 GB/s each, which is the HBM's rate (32 x n x 16384, whole tiles, weights larger than L2 in
+// turn: 40 to 42 us for 18, 37 and 74 tiles, 43 for 111, 53 for 148). So a few long tiles are shared out by k, to
 // 128 bytes evenly: the CTAs of a tile leave int32 sums in the workspace, and the last of them to finish adds them.
 // k_int8_pair: persistent CTA pairs (cta_group::2) on 256 x 256 tiles with two accumulators in
 // TMEM, so the epilogue of one tile runs under the products of the next.
@@ -526,12 +527,12 @@ int launch_cluster(tb_ctx* ctx, const char* what, dim3 grid, int threads, int sm
 int shared_tokens(int64_t m) { return (int)round_up(ceil_div(m, ceil_div(m, 128)), 16); }
 
 // How a product is run: the fastest of three by what they were measured to take, us, for `ktiles` steps of 128 bytes
-// of k. Whole tiles of one CTA, 4.5 + 0.34 a step and wave: an SM takes that for a step whatever its tokens, the weights' 16 KB at
-// 48 bytes a nanosecond; so the tokens go in as many tiles as one wave holds, which shortens the epilogues (128 x
-// 4096 x 4096: 14.3 on tiles of 32 tokens, 15.0 of 128). One wave of tiles at most, shared out by k evenly over all SMs: 6 and
-// 0.04 a token of the tile more, to leave and add the partial sums (32 x 4096 x 16384: 21 shared, 48 whole; 128 x
+// of k. Whole tiles of one CTA, 4.5 + 0.34 a step and wave: an SM takes that for a step's 16 KB of weights whatever its tokens
+// (0.28 where few SMs have a tile, 0.38 where all have); so the tokens go in as many tiles as one wave holds, which shortens the epilogues (128 x
+// 4096 x 4096: 13.6 on tiles of 32 tokens, 14.6 of 128). One wave of tiles at most, shared out by k evenly over all SMs: 6 and
+// 0.04 a token of the tile more, to leave and add the partial sums (32 x 4096 x 16384: 20 shared, 41 whole; 128 x
 // 4096 x 4096: 18 shared). Tiles of CTA pairs, 7.5 + 0.36 a step and wave for four times the work (1000 x 4096 x
-// 4096: 19, and 26 in whole tiles; 512 x 4096 x 4096: 19 and 16).
+// 4096: 19, and 25 in whole tiles; 512 x 4096 x 4096: 18 and 16).
 struct Plan {
     int bt;        // tokens of a tile of the single-CTA kernel, 0 for pairs
     bool share;

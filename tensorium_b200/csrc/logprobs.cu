@@ -456,13 +456,13 @@ __device__ __forceinline__ void take(unsigned long long& list, unsigned long lon
 // One pass over the logits. NW warps to a row, or to one of `splits` parts of it; where a warp has a row to itself, four to a
 // CTA. Each step of a thread is a group of U chunks; the groups' maxima stay in shared memory, so that after the
 // pass only the groups that can hold one of the best are read again: those whose maximum reaches the k-th largest of
-// the threads' maxima, about k of them. Lists kept during the pass took 530 us for 4096 x 131072 bf16 top 20, this 198
-// (5.4 TB/s), and 172 (6.3 TB/s) without alternatives; what is left of the difference is the chain at a row's end,
+// the threads' maxima, about k of them. Lists kept during the pass took 530 us for 4096 x 131072 bf16 top 20, this 194
+// (5.5 TB/s), and 168 (6.4 TB/s) without alternatives; what is left of the difference is the chain at a row's end,
 // which the other CTAs of an SM cover in part. Few rows in parts: 1 x 131072 top 20 in 7.8 us, the latency of two rounds to memory
-// and of joining the parts.
+// and of joining the parts. (Times in this file: of the kernel, in a graph of calls on inputs larger than L2 together.)
 constexpr int LP_U = 4;
 // Most steps of a part: a CTA's groups fit its shared memory, and longer rows are faster on more warps (4096 x 131072 bf16 top
-// 20: 198 us on 4, 222 on 2).
+// 20: 194 us on 4, 217 on 2, 201 on 8).
 template <typename T> int lp_steps(int nw) { return nw < 8 ? 40 : sizeof(T) == 4 ? 28 : 32; }
 
 constexpr int KEYS = 64;  // candidates that are ranked against one another
@@ -787,11 +787,11 @@ template <typename T> int launch_logprobs(tb_ctx* ctx, LogprobArgs p) {
     const int64_t chunks = ceil_div(p.vocab + (aligned ? 0 : E - 1), E);
     const int64_t step = 32 * LP_U;                   // chunks a step of one warp
     // Warps per row: the fewest (a row's end keeps few of them busy) that put 20 warps on every SM and leave a part
-    // within lp_steps() steps. Measured with 1 / 2 / 4 / 8 warps, us: 8192 x 2048 bf16 top 5 18.7 / 25.7 / 47 / 88, 4096 x 32000 60 / 63 / 65 /
-    // 77, 1000 x 16000 22.8 / 16.3 / 13.7 / 17.6, 777 x 30001 f32 46 / 27.8 / 19.9 / 23.0.
+    // within lp_steps() steps. Measured with 1 / 2 / 4 / 8 warps, us: 8192 x 2048 bf16 top 5 16.6 / 22.1 / 35 / 65, 4096 x 32000 60 / 59 / 62 /
+    // 82, 1000 x 16000 16.2 / 16.2 / 12.9 / 15.8, 777 x 30001 f32 - / 27.0 / 20.7 / 24.4.
     // Short rows share warps where they fill the GPU that way, or need no alternatives (else a warp to a row has the shorter
-    // chain, and finds more of them): 16384 x 1000 f16 top 5 in 14.9 us and 21.0 with a warp each, 16384 x 80 7.2 and
-    // 17.7, 60000 x 10 14.2 and 65.6; 200 x 200 4.7 and 4.0.
+    // chain, and finds more of them): 16384 x 1000 f16 top 5 in 14.9 us and 20.5 with a warp each, 16384 x 80 7.0 and
+    // 17.3, 60000 x 10 14.4 and 64; 200 x 200 4.6 and 4.0.
     const int lanes = chunks <= 4 * SHORT_U && p.top <= 4 ? 4 : chunks <= 8 * SHORT_U ? 8 : chunks <= 16 * SHORT_U ? 16 : 32;
     if (chunks <= lanes * SHORT_U && p.top <= SHORT_TOP && (p.top == 0 || p.rows * lanes / 32 >= 8 * ctx->sm_count)) {
         auto run = [&](auto n) {
@@ -808,8 +808,8 @@ template <typename T> int launch_logprobs(tb_ctx* ctx, LogprobArgs p) {
     int nw = 1;
     while (nw < 8 && chunks > step * nw && (p.rows * nw < 20 * ctx->sm_count || chunks > step * nw * lp_steps<T>(nw))) nw *= 2;
     // With 8, few rows go in parts: of one step while all of them have an SM each, else of two steps at least and two CTAs
-    // to an SM at most (1 x 131072 bf16 top 20 7.7 us in 16 parts, 8.1 in 8; 48 x 50001 f32 top 5 10.7 in 6, 11.7 in 12). Joining them
-    // costs what up to 6 steps take (8 x 32000 bf16 top 5 6.3 whole, 7.4 in 4 parts; 5 x 60000 8.1 and 7.4).
+    // to an SM at most (1 x 131072 bf16 top 20 7.7 us in 16 parts, 8.1 in 8; 48 x 50001 f32 top 5 10.4 in 6, 11.4 in 12). Joining them
+    // costs what up to 6 steps take (8 x 32000 bf16 top 5 6.3 whole, 7.4 in 4 parts; 5 x 60000 8.5 whole, 7.4 in 8).
     const int64_t steps = ceil_div(chunks, step * nw), sms = ctx->sm_count;
     int64_t splits = 1;
     if (nw == 8) {
@@ -817,8 +817,8 @@ template <typename T> int launch_logprobs(tb_ctx* ctx, LogprobArgs p) {
         splits = std::max<int64_t>({1, std::min<int64_t>(splits, 256), ceil_div(steps, lp_steps<T>(nw))});
     }
     p.splits = (int)splits;
-    // From 3 steps on the next step's loads are taken under this one's sums (777 x 50001 f32 33 -> 28 us), with 24 warps to an SM
-    // instead of 32: not where that makes a second wave (4096 x 32000 with a warp a row 60 -> 72 us).
+    // From 3 steps on the next step's loads are taken under this one's sums (777 x 50001 f32 31 -> 28 us), with 24 warps to an SM
+    // instead of 32: not where that makes a second wave (4096 x 32000 with a warp a row 59 -> 67 us).
     const int64_t warps = p.rows * splits * nw;
     const bool ahead = ceil_div(steps, splits) >= 3 && (warps <= 24 * sms || warps > 32 * sms);
     p.steps = (int)ceil_div(steps, p.splits);
@@ -868,7 +868,7 @@ struct LogprobBwdArgs {
 };
 
 // d = (a (delta - p) - b p (log p + h)) / T, log p = (l - max) / T - log_sum. Memory bound: 4096 x 131072 bf16 in
-// 306 us (7.0 TB/s), 346 in a second of such calls, where a copy of as many bytes takes 333. A CTA takes 4 x 256 chunks of a row, or (WARP) each
+// 308 us (7.0 TB/s); a copy of as many bytes takes 333, in a second of copies. A CTA takes 4 x 256 chunks of a row, or (WARP) each
 // of its warps a row of up to 4 x 32. In place is safe: a thread writes the chunks that it has read.
 template <typename T, bool WARP> __global__ void __launch_bounds__(256) k_token_logprobs_bwd(const LogprobBwdArgs p) {
     TB_GRID_DEP_ENTRY();
